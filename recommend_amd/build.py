@@ -16,6 +16,9 @@ FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-fno-fast-math", "-ffp-contract=off",
     "-fhip-fp32-correctly-rounded-divide-sqrt",
+    # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on this hardware now and
+    # then (hipcc's host pass does not know the feature and says so: harmless)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function", "-Wno-inline-asm",
 ]
 
