@@ -20,7 +20,8 @@
  *    owned by the caller; the library allocates no device memory;
  *  - `stream` is a hipStream_t passed as void*; all device work is enqueued
  *    asynchronously on it and the functions do not synchronise;
- *  - dense matrices are row-major fp32, 16-byte aligned rows; graph indices
+ *  - dense matrices are row-major fp32, 16-byte aligned rows, unless an entry
+ *    point takes an element type (then any alignment of whole elements); graph indices
  *    are int32 on the device (node count and nnz < 2^31); batch ids are
  *    int64 as the reference's batch dict holds them.
  */
@@ -41,6 +42,11 @@ extern "C" {
 #define RK_ERR_NODEV (-4)       /* no gfx950 device visible                 */
 
 #define RK_ABI_VERSION 1
+
+/* element types of the entry points that take more than fp32 */
+#define RK_F32 0
+#define RK_BF16 1
+#define RK_F16 2
 
 /* ---- library ---------------------------------------------------------- */
 int rk_abi_version(void);
@@ -316,6 +322,101 @@ int rk_adam_update_f32(const rk_adam_tensor *tensors_host, int32_t n_tensors, in
                        const int64_t *step, const float *lr, float beta1, float beta2, float eps,
                        float weight_decay, float max_norm, const float *shard_sq, float *norm_out,
                        const void *ws, size_t ws_bytes, void *stream);
+
+/* ---- embedding lookup with scaling, and its gradient ---------------------- */
+/* The nn.Embedding lookups of the reference's models (model/Main_Model.py:79,98) with a factor:
+ * out[i, :] = scale * weight[ids[i], :] (product in fp32, rounded once to the table's type).
+ * weight: rows x D of element type dtype (RK_F32 / RK_BF16 / RK_F16), ld_weight elements between
+ * rows; any D >= 1 and any alignment of whole elements.  ids: n int32 (id_bytes 4) or int64 (8).
+ * An id outside [0, rows) reads nothing and gives a row of NaN. */
+int rk_embedding_fwd(const void *weight, int64_t ld_weight, int32_t rows, int32_t D, int32_t dtype,
+                     const void *ids, int32_t id_bytes, int64_t n, float scale, void *out, void *stream);
+/* d_weight[v, :] = scale * sum over { i : ids[i] = v } of grad[i, :], every row of d_weight written
+ * (zeros where no id names it).  grad: n x D, d_weight: rows x D, both contiguous, of type dtype.  Sums
+ * in fp32, in an order that depends on the ids alone (no floating atomics): the same bits on every
+ * run.  Positions whose id is padding_idx or outside [0, rows) add nothing (padding_idx < 0: none).
+ * ws: rk_embedding_bwd_ws_bytes() bytes of scratch. */
+size_t rk_embedding_bwd_ws_bytes(int64_t n, int32_t rows, int32_t D, int32_t dtype);
+int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t id_bytes, int64_t n,
+                     int32_t rows, int32_t D, float scale, int64_t padding_idx, void *d_weight,
+                     void *ws, size_t ws_bytes, void *stream);
+
+/* ---- log-probabilities of item lists; preference loss of pairs of lists ---- */
+/* No counterpart in the reference; its pairwise losses (evalue/loss.py:7-28) are the special case of
+ * one place and a constant reference model.  scores: S lists x T places x V catalogue items of type
+ * dtype, element (s, t, j) at s * stride_s + t * stride_t + j; items: int64 [S, T] with ld_items
+ * between lists: the item at a place, or ignore_index where the place is not in use.
+ *   logps[s] = sum_t (x[s, t, items[s, t]] - log sum_j exp x[s, t, j])   over the places in use
+ * (average != 0: divided by their number; a list without any has 0).  Places that are not in use
+ * are not read.  An item outside [0, V) makes its list's result NaN.  stat: [S * T][2] floats and
+ * used: [S] int32, kept for the backward call.  ws: rk_list_logps_ws_bytes() bytes of scratch. */
+size_t rk_list_logps_ws_bytes(int32_t S, int32_t T, int32_t V);
+int rk_list_logps_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, int32_t V,
+                      int64_t stride_s, int64_t stride_t, const int64_t *items, int64_t ld_items,
+                      int64_t ignore_index, int32_t average, float *stat, float *logps, int32_t *used,
+                      void *ws, size_t ws_bytes, void *stream);
+/* The same with the loss of the pairs (p, S/2 + p), the preferred list first:
+ *   d = (logps[p] - ref_logps[p]) - (logps[S/2 + p] - ref_logps[S/2 + p])
+ *   RK_PREF_SIGMOID  (1 - e) softplus(-beta d) + e softplus(beta d)     e = label_smoothing
+ *   RK_PREF_HINGE    max(0, 1 - beta d)
+ *   RK_PREF_SQUARED  (d - 1 / (2 beta))^2
+ * loss[0]: their mean; slope: [S] floats, d loss / d logps, kept for the backward call. */
+#define RK_PREF_SIGMOID 0
+#define RK_PREF_HINGE 1
+#define RK_PREF_SQUARED 2
+int rk_preference_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, int32_t V,
+                      int64_t stride_s, int64_t stride_t, const int64_t *items, int64_t ld_items,
+                      int64_t ignore_index, int32_t average, const float *ref_logps, float beta,
+                      float label_smoothing, int32_t kind, float *stat, float *logps, int32_t *used,
+                      float *slope, float *loss, void *ws, size_t ws_bytes, void *stream);
+/* d_scores [S, T, V] (contiguous, of type dtype) for the gradients g_loss (one float; may be NULL) of
+ * the loss and g_logps ([S]; may be NULL) of the log-probabilities; zeros at places not in use. */
+int rk_list_logps_bwd(const void *scores, int32_t dtype, int32_t S, int32_t T, int32_t V,
+                      int64_t stride_s, int64_t stride_t, const int64_t *items, int64_t ld_items,
+                      int64_t ignore_index, int32_t average, const float *stat, const int32_t *used,
+                      const float *g_loss, const float *slope, const float *g_logps, void *d_scores,
+                      void *stream);
+
+/* ---- AdamW over many tensors, moments in 32 or 8 bits ---------------------- */
+/* The reference's AdamW choice (train/graph_trainer.py:78-101) with clip_grad_norm_ (:151-156), in two
+ * launches per 48 tensors; nothing is allocated, so a call can be recorded in a HIP graph.
+ *   g = min(1, max_norm / (|grads| + 1e-6)) * grad           (max_norm <= 0: no clipping)
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p - lr wd p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * param / grad: n elements of param_dtype / grad_dtype (the parameter's type or RK_F32).
+ * exp_avg / exp_avg_sq: fp32 moments when both scales are NULL.  Otherwise 8-bit moments: e4m3 codes
+ * of m and of sqrt(v), padded to whole blocks of RK_ADAMW_BLOCK elements, with one fp32 scale per
+ * block: value = code * scale, the block's largest magnitude at code 448, rounded to nearest; a
+ * sqrt(v) that is not zero is at least the smallest code.
+ * lr: device array of n_groups floats; step: device counter, incremented by the call; norm_out (may
+ * be NULL): the gradients' 2-norm before clipping, written when max_norm > 0.  ws:
+ * rk_adamw_ws_bytes() bytes, 16-byte aligned, zeroed once by the caller and left ready for the next
+ * call; calls that share it must not overlap in time. */
+#define RK_ADAMW_BLOCK 64
+#define RK_ADAMW_MAX_GROUPS 8
+typedef struct rk_adamw_tensor {
+  void *param;
+  const void *grad;
+  void *exp_avg;
+  void *exp_avg_sq;
+  float *exp_avg_scale;
+  float *exp_avg_sq_scale;
+  int64_t n;
+  int32_t param_dtype;
+  int32_t grad_dtype;
+  int32_t group;
+  int32_t reserved;
+} rk_adamw_tensor;
+typedef struct rk_adamw_group {
+  double beta1;
+  double beta2;
+  double eps;
+  double weight_decay;
+} rk_adamw_group;
+size_t rk_adamw_ws_bytes(int32_t n_tensors);
+int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors,
+                  const rk_adamw_group *groups_host, int32_t n_groups, int64_t *step, const float *lr,
+                  float max_norm, float *norm_out, void *ws, size_t ws_bytes, void *stream);
 
 /* ---- N: negative sampling (host RNG, bit-exact) ------------------------- */
 /* Replaces GraphDataLoader._generate_negative_samples,

@@ -34,6 +34,23 @@ class AdamTensor(Structure):
                 ("n", c_int64)]
 
 
+# element types of the entry points that take more than fp32 (RK_F32, RK_BF16, RK_F16)
+F32, BF16, F16 = 0, 1, 2
+
+ADAMW_BLOCK = 64
+ADAMW_MAX_GROUPS = 8
+
+
+class AdamwTensor(Structure):
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p),
+                ("exp_avg_scale", c_void_p), ("exp_avg_sq_scale", c_void_p), ("n", c_int64),
+                ("param_dtype", c_int32), ("grad_dtype", c_int32), ("group", c_int32), ("reserved", c_int32)]
+
+
+class AdamwGroup(Structure):
+    _fields_ = [("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double)]
+
+
 class SpmmPlan(Structure):
     _fields_ = [
         ("long_thresh", c_int32),
@@ -109,6 +126,19 @@ SIGNATURES = {
     "rk_adam_sqnorm_f32": (c_int32, [P, c_int32, c_int32, P, P, P, c_size_t, P]),
     "rk_adam_update_f32": (c_int32, [P, c_int32, c_int32, P, P, c_float, c_float, c_float, c_float, c_float, P, P, P,
                                      c_size_t, P]),
+    "rk_embedding_fwd": (c_int32, [P, c_int64, c_int32, c_int32, c_int32, P, c_int32, c_int64, c_float, P, P]),
+    "rk_embedding_bwd_ws_bytes": (c_size_t, [c_int64, c_int32, c_int32, c_int32]),
+    "rk_embedding_bwd": (c_int32, [P, c_int32, P, c_int32, c_int64, c_int32, c_int32, c_float, c_int64, P, P,
+                                   c_size_t, P]),
+    "rk_list_logps_ws_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "rk_list_logps_fwd": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, P, c_int64, c_int64,
+                                    c_int32, P, P, P, P, c_size_t, P]),
+    "rk_preference_fwd": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, P, c_int64, c_int64,
+                                    c_int32, P, c_float, c_float, c_int32, P, P, P, P, P, P, c_size_t, P]),
+    "rk_list_logps_bwd": (c_int32, [P, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64, P, c_int64, c_int64,
+                                    c_int32, P, P, P, P, P, P, P]),
+    "rk_adamw_ws_bytes": (c_size_t, [c_int32]),
+    "rk_adamw_step": (c_int32, [P, c_int32, P, c_int32, P, P, c_float, P, P, c_size_t, P]),
     "rk_mt_seed_host": (c_int32, [P, c_uint64]),
     "rk_neg_sample_host": (c_int32, [P, P, c_int64, c_int32, P, P, c_int32, P, P]),
     "rk_neg_order_host": (c_int32, [P, c_int32, c_int32, P]),
@@ -202,11 +232,22 @@ def ptr(t):
     return c_void_p(t.ctypes.data)
 
 
+def call_on(device, name, *args):
+    """`call` with `device` current: a launch goes to the device its stream belongs to."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
 def stream_ptr(device=None):
     import torch
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-__all__ = ["load", "call", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "RkError", "SIGNATURES",
+__all__ = ["load", "call", "call_on", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "AdamwTensor", "AdamwGroup",
+           "RkError", "SIGNATURES",
            "LIB_PATH", "device_count", "require_device", "last_error",
            "c_int32", "c_int64", "c_float", "c_double", "c_uint32", "c_size_t"]

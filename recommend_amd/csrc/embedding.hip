@@ -1,0 +1,614 @@
+// Embedding lookup with scaling, out[i] = scale * weight[ids[i]], and its gradient by sorted ids,
+//   dW[v] = scale * sum over { i : ids[i] = v } of g[i]        (gfx950).
+//
+// The gradient never adds with floating atomics.  The ids are sorted together with their positions
+// (stable: equal ids keep the order of their positions), so a row's contributions lie side by side;
+// lane groups add them in registers in that order and write each row of dW once.  The sums are fp32
+// whatever the tensors' type, the same bits on every run, and rounded once.
+//
+// Sort: up to kRankSortMax ids one launch counts, for every id, the ids that come before it.  More
+// ids take an LSD radix sort with digits of up to 9 bits: per digit one launch that counts a tile's
+// digits and one that places them (every workgroup adds up the counts in front of its own itself).
+// Padded and out-of-range ids get the key `rows`: they come last and add nothing.
+//
+// Sum: a lane group takes `per_group` consecutive sorted entries and keeps the running row in
+// registers.  A row that begins and ends inside the group's entries is written at once; the pieces
+// of rows that cross groups are joined in LDS, and the pieces that cross workgroups through memory
+// by the closing launch, in the order of the entries.  Rows without an entry are zeroed by further
+// workgroups of the same launch, which look their ids up in the sorted keys.
+#include <algorithm>
+
+#include "elem.h"
+
+namespace {
+
+constexpr int kRankSortMax = 4096;    // ids sorted by counting
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / rk::kWave;
+constexpr int kMaxDigitBits = 9;
+constexpr int kMaxTiles = 128;        // tiles of a radix pass: every workgroup adds up this many counts per digit
+constexpr int kMinTile = 8192;
+constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
+constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
+constexpr int kLongRun = 32;          // workgroup pieces of a row above which a whole workgroup joins them
+
+// the sort key of an id: ids outside [0, rows) and the padding id go behind all rows
+template <typename ID>
+__device__ __forceinline__ int32_t key_of(ID id, int32_t rows, int64_t padding) {
+  return (id < 0 || (int64_t)id >= rows || (int64_t)id == padding) ? rows : (int32_t)id;
+}
+
+// ------------------------------------------------------------------------------------- lookup
+template <typename T, int VEC, typename ID>
+__global__ __launch_bounds__(256) void emb_fwd_kernel(const T *__restrict__ W, int64_t ldw, int32_t rows, int32_t D,
+                                                      const ID *__restrict__ ids, int64_t n, float scale, int32_t L,
+                                                      int32_t per_thread, T *__restrict__ out) {
+  const int G = 256 / L, grp = threadIdx.x / L, l = threadIdx.x - grp * L;
+  if (grp >= G) return;
+  const int64_t base = (int64_t)blockIdx.x * G * per_thread;
+  for (int c0 = 0; c0 < D; c0 += L * VEC) {
+    if (c0 + l * VEC >= D) break;
+    const int col = min(c0 + l * VEC, D - VEC);   // the last vector of a row overlaps the one before it
+    for (int r0 = 0; r0 < per_thread; r0 += 4) {
+      rk::Pack<T, VEC> v[4];
+      bool ok[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t i = base + (int64_t)(r0 + j) * G + grp;
+        const ID id = r0 + j < per_thread && i < n ? ids[i] : (ID)-1;
+        ok[j] = id >= 0 && (int64_t)id < rows;
+        if (ok[j]) v[j].load(W + (int64_t)id * ldw + col);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t i = base + (int64_t)(r0 + j) * G + grp;
+        if (r0 + j >= per_thread || i >= n) continue;
+        float x[VEC];
+        if (ok[j]) {
+          v[j].widen(x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x[e] *= scale;
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) x[e] = __builtin_nanf("");   // no row has this id
+        }
+        v[j].narrow(x);
+        v[j].store(out + i * D + col);
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------- sort
+// position of id i = number of ids in front of it: smaller keys, and equal keys at lower positions.
+// 32 ids per workgroup, eight threads each.
+template <typename ID>
+__global__ __launch_bounds__(256) void emb_rank_sort_kernel(const ID *__restrict__ ids, int32_t n, int32_t rows,
+                                                            int64_t padding, int32_t *__restrict__ keys,
+                                                            int32_t *__restrict__ perm) {
+  __shared__ int32_t s_key[kRankSortMax];
+  for (int j = threadIdx.x; j < n; j += 256) s_key[j] = key_of(ids[j], rows, padding);
+  __syncthreads();
+  const int i = blockIdx.x * 32 + threadIdx.x / 8, sub = threadIdx.x % 8;
+  const int32_t my = i < n ? s_key[i] : 0;
+  int before = 0;
+  if (i < n)
+    for (int j = sub; j < n; j += 8) before += s_key[j] < my + (j < i ? 1 : 0);
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) before += __shfl_xor(before, off, 8);
+  if (i < n && sub == 0) {
+    keys[before] = my;
+    perm[before] = i;
+  }
+}
+
+// source of a radix pass: the ids themselves (first pass) or the keys and positions of the last pass
+template <typename ID>
+struct FromIds {
+  const ID *ids;
+  int32_t rows;
+  int64_t padding;
+  __device__ __forceinline__ int32_t key(int32_t i) const { return key_of(ids[i], rows, padding); }
+  __device__ __forceinline__ int32_t pos(int32_t i) const { return i; }
+};
+struct FromPass {
+  const int32_t *keys, *perm;
+  __device__ __forceinline__ int32_t key(int32_t i) const { return keys[i]; }
+  __device__ __forceinline__ int32_t pos(int32_t i) const { return perm[i]; }
+};
+
+template <typename SRC>
+__global__ __launch_bounds__(kSortThreads) void emb_count_kernel(SRC src, int32_t n, int32_t tile, int shift, int bits,
+                                                                 int32_t *__restrict__ counts) {
+  __shared__ int32_t s_count[1 << kMaxDigitBits];
+  const int nd = 1 << bits;
+  for (int d = threadIdx.x; d < nd; d += kSortThreads) s_count[d] = 0;
+  __syncthreads();
+  const int32_t lo = (int32_t)blockIdx.x * tile, hi = (int32_t)min((int64_t)n, (int64_t)lo + tile);
+  for (int32_t i = lo + threadIdx.x; i < hi; i += kSortThreads)
+    atomicAdd(&s_count[(src.key(i) >> shift) & (nd - 1)], 1);
+  __syncthreads();
+  for (int d = threadIdx.x; d < nd; d += kSortThreads) counts[(int64_t)blockIdx.x * nd + d] = s_count[d];
+}
+
+// Places one tile: every wavefront owns a consecutive part of it, so that (wavefront, step, lane) is the
+// order of the positions and equal digits keep it.
+template <typename SRC>
+__global__ __launch_bounds__(kSortThreads) void emb_place_kernel(SRC src, int32_t n, int32_t tile, int shift, int bits,
+                                                                 const int32_t *__restrict__ counts,
+                                                                 int32_t *__restrict__ keys, int32_t *__restrict__ perm) {
+  extern __shared__ int32_t s_off[];   // [kSortWaves][nd]: next place of a digit for every wavefront
+  __shared__ int32_t s_total[1 << kMaxDigitBits], s_front[1 << kMaxDigitBits], s_wave[kSortWaves];
+  const int nd = 1 << bits, t = threadIdx.x, wave = t / rk::kWave, lane = t % rk::kWave;
+  for (int i = t; i < kSortWaves * nd; i += kSortThreads) s_off[i] = 0;
+  for (int d = t; d < nd; d += kSortThreads) s_total[d] = s_front[d] = 0;
+  __syncthreads();
+  // counts of every digit over all tiles and over the tiles in front of this one (integer sums: any order)
+  const int my_tile = blockIdx.x, n_tiles = gridDim.x, parts = kSortThreads / nd;
+  {
+    const int d = t & (nd - 1), part = t / nd;
+    int32_t total = 0, front = 0;
+    for (int k = part; k < n_tiles; k += parts) {
+      const int32_t c = counts[(int64_t)k * nd + d];
+      total += c;
+      front += k < my_tile ? c : 0;
+    }
+    atomicAdd(&s_total[d], total);
+    atomicAdd(&s_front[d], front);
+  }
+  // digits of every wavefront's part of the tile
+  const int32_t part_len = tile / kSortWaves;
+  const int64_t end = min((int64_t)n, (int64_t)my_tile * tile + tile);
+  const int64_t lo = (int64_t)my_tile * tile + (int64_t)wave * part_len;
+  const int64_t hi = min(end, lo + part_len);
+  for (int64_t i = lo + lane; i < hi; i += rk::kWave)
+    atomicAdd(&s_off[wave * nd + ((src.key((int32_t)i) >> shift) & (nd - 1))], 1);
+  __syncthreads();
+  // exclusive sum over the digits (nd <= kSortThreads), then over the wavefronts of this tile
+  int32_t total = t < nd ? s_total[t] : 0, incl = total;
+#pragma unroll
+  for (int off = 1; off < rk::kWave; off <<= 1) {
+    const int32_t o = __shfl_up(incl, off, rk::kWave);
+    if (lane >= off) incl += o;
+  }
+  if (lane == rk::kWave - 1) s_wave[wave] = incl;
+  __syncthreads();
+  if (t < nd) {
+    int32_t at = incl - total + s_front[t];
+    for (int w = 0; w < wave; ++w) at += s_wave[w];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int32_t c = s_off[w * nd + t];
+      s_off[w * nd + t] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+  for (int64_t i0 = lo; i0 < hi; i0 += rk::kWave) {
+    const int64_t i = i0 + lane;
+    const bool in = i < hi;
+    const int32_t key = in ? src.key((int32_t)i) : 0, pos = in ? src.pos((int32_t)i) : 0;
+    const int d = (key >> shift) & (nd - 1);
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? set : ~set;
+    }
+    if (in) {
+      const int rank = __popcll(same & ((1ull << lane) - 1));
+      const int32_t at = s_off[wave * nd + d] + rank;
+      keys[at] = key;
+      perm[at] = pos;
+    }
+    // (a wavefront's LDS operations complete in program order: all lanes have read before one writes)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (in && (same >> lane) == 1) s_off[wave * nd + d] += __popcll(same);   // the last lane with this digit
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// ---------------------------------------------------------------------------------------- sum
+struct SumArgs {
+  const int32_t *keys, *perm;   // sorted ids and where they stood
+  int32_t n, rows, D;
+  int32_t L, G, per_group;      // lanes of a row, rows side by side in a workgroup, entries of a lane group
+  int32_t blocks;               // workgroups that sum; the ones behind them zero
+  float scale;
+  float *pieces;                // [blocks][2][D]: what a workgroup has of the row it begins / ends in
+};
+
+// first place of a key that is not below v
+__device__ __forceinline__ int32_t lower_bound(const int32_t *__restrict__ keys, int32_t n, int32_t v) {
+  int32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_rows(const SumArgs &a, int32_t z, T *__restrict__ dW) {
+  const int32_t v = z * kZeroRows + (int32_t)threadIdx.x;
+  bool absent = false;
+  if (v < a.rows) {
+    const int32_t at = lower_bound(a.keys, a.n, v);
+    absent = !(at < a.n && a.keys[at] == v);
+  }
+  const uint64_t mask = __ballot(absent);
+  if (!mask) return;
+  const int lane = threadIdx.x % rk::kWave, per_row = (a.D + VEC - 1) / VEC;
+  const int64_t row0 = (int64_t)z * kZeroRows + (threadIdx.x - lane);
+  rk::Pack<T, VEC> zero;
+#pragma unroll
+  for (int i = 0; i < rk::Pack<T, VEC>::kWords; ++i) zero.w[i] = 0u;
+  for (int i = lane; i < rk::kWave * per_row; i += rk::kWave) {
+    const int r = i / per_row;
+    if ((mask >> r) & 1) zero.store(dW + (row0 + r) * a.D + min((i - r * per_row) * VEC, a.D - VEC));
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void put_row(T *__restrict__ dst, const float (&acc)[VEC], float scale) {
+  float x[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) x[e] = acc[e] * scale;
+  rk::Pack<T, VEC> v;
+  v.narrow(x);
+  v.store(dst);
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__restrict__ g, T *__restrict__ dW) {
+  constexpr int U = 8;                                   // rows of g in flight per lane group
+  __shared__ int32_t s_key[kMaxEntries + 2];             // [0]: the key in front, [1 + count]: the key behind
+  __shared__ int32_t s_pos[kMaxEntries];
+  __shared__ float s_head[256 * VEC], s_tail[256 * VEC]; // what a group has of the row it begins / ends in
+  __shared__ uint8_t s_through[256], s_has_tail[256];
+  if ((int32_t)blockIdx.x >= a.blocks) {
+    zero_rows<T, VEC>(a, (int32_t)blockIdx.x - a.blocks, dW);
+    return;
+  }
+  const int per_block = a.G * a.per_group;
+  const int32_t s0 = (int32_t)blockIdx.x * per_block, s1 = (int32_t)min((int64_t)a.n, (int64_t)s0 + per_block);
+  int count = s1 - s0;
+  for (int i = threadIdx.x; i < count; i += 256) {
+    s_key[1 + i] = a.keys[s0 + i];
+    s_pos[i] = a.perm[s0 + i];
+  }
+  if (threadIdx.x == 0) {
+    s_key[0] = s0 > 0 ? a.keys[s0 - 1] : -1;
+    s_key[1 + count] = s1 < a.n ? a.keys[s1] : -1;
+  }
+  __syncthreads();
+  if (s_key[count] >= a.rows) count = lower_bound(s_key + 1, count, a.rows);   // entries that add nothing come last
+  if (count == 0) return;
+  const int grp = threadIdx.x / a.L, l = threadIdx.x - grp * a.L;
+  const int es = min(count, grp * a.per_group), ee = min(count, es + a.per_group);
+  const bool live = grp < a.G && es < ee;
+  const bool began_before = live && s_key[es] == s_key[1 + es];
+
+  for (int c0 = 0; c0 < a.D; c0 += a.L * VEC) {
+    const bool on = live && c0 + l * VEC < a.D;
+    const int col = min(c0 + l * VEC, a.D - VEC), slot = threadIdx.x * VEC;
+    bool through = false, has_tail = false;
+    if (on) {
+      float acc[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+      int32_t cur = s_key[1 + es];
+      bool first = began_before;                         // still in the row that an earlier group began
+      for (int i = es; i < ee; i += U) {
+        rk::Pack<T, VEC> v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) v[j].load(g + (int64_t)s_pos[min(i + j, ee - 1)] * a.D + col);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          if (i + j >= ee) break;
+          const int32_t k = s_key[1 + i + j];
+          if (k != cur) {
+            if (first) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) s_head[slot + e] = acc[e];
+            } else {
+              put_row<T, VEC>(dW + (int64_t)cur * a.D + col, acc, a.scale);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+            cur = k;
+            first = false;
+          }
+          float x[VEC];
+          v[j].widen(x);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += x[e];
+        }
+      }
+      const bool goes_on = s_key[1 + ee] == cur;
+      if (first) {
+        through = goes_on;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_head[slot + e] = acc[e];
+      } else if (goes_on) {
+        has_tail = true;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_tail[slot + e] = acc[e];
+      } else {
+        put_row<T, VEC>(dW + (int64_t)cur * a.D + col, acc, a.scale);
+      }
+    }
+    if (l == 0 && grp < a.G) {
+      s_through[grp] = through;
+      s_has_tail[grp] = has_tail;
+    }
+    __syncthreads();
+    if (on && s_has_tail[grp]) {                         // a row begins here and goes on: add the groups behind
+      float acc[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = s_tail[slot + e];
+      int j = grp + 1;
+      bool open = true;
+      for (; j < a.G && open; ++j) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += s_head[(j * a.L + l) * VEC + e];
+        open = s_through[j];
+      }
+      if (!open) {
+        put_row<T, VEC>(dW + (int64_t)s_key[ee] * a.D + col, acc, a.scale);
+      } else {
+        float *p = a.pieces + ((int64_t)blockIdx.x * 2 + 1) * a.D + col;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+      }
+    }
+    if (on && grp == 0 && began_before) {                // the row that an earlier workgroup began
+      float acc[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = s_head[slot + e];
+      for (int j = 0; s_through[j] && j + 1 < a.G; ++j) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += s_head[((j + 1) * a.L + l) * VEC + e];
+      }
+      float *p = a.pieces + (int64_t)blockIdx.x * 2 * a.D + col;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) p[e] = acc[e];
+    }
+    __syncthreads();
+  }
+}
+
+// Rows that cross workgroups: the workgroup in which such a row begins has a tail piece, the ones it
+// goes on into have head pieces; they are added in that order.  One lane group per workgroup of the
+// summing launch; rows with many pieces are added by the whole workgroup, a consecutive share each.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict__ dW) {
+  __shared__ float s_part[256 * VEC];
+  __shared__ int32_t s_last[256];                        // last workgroup of the row that begins in this one (0: none)
+  const int per_block = a.G * a.per_group;
+  const int grp = threadIdx.x / a.L, l = threadIdx.x - grp * a.L;
+  const int32_t b = (int32_t)blockIdx.x * a.G + grp;
+  int32_t last = 0;
+  if (grp < a.G && (int64_t)(b + 1) * per_block < a.n) {
+    const int32_t s0 = b * per_block, s1 = s0 + per_block, key = a.keys[s1 - 1];
+    const bool goes_on = key < a.rows && a.keys[s1] == key;
+    const bool began_before = s0 > 0 && a.keys[s0 - 1] == key;
+    if (goes_on && !began_before) {
+      const int32_t end = s1 + lower_bound(a.keys + s1, min(a.n - s1, per_block + 1), key + 1);
+      last = b + 1;
+      if (end - s1 > per_block) {                        // beyond the next workgroup: look for its end
+        const int32_t far = s1 + lower_bound(a.keys + s1, a.n - s1, key + 1);
+        last = (far - 1) / per_block;
+      }
+    }
+  }
+  if (grp < a.G && l == 0) s_last[grp] = last;
+  __syncthreads();
+  for (int c0 = 0; c0 < a.D; c0 += a.L * VEC) {
+    const bool on = grp < a.G && c0 + l * VEC < a.D;
+    const int col = min(c0 + l * VEC, a.D - VEC);
+    if (on && last > 0 && last - b <= kLongRun) {
+      float acc[VEC];
+      const float *p = a.pieces + ((int64_t)b * 2 + 1) * a.D + col;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] = p[e];
+      for (int32_t k = b + 1; k <= last; ++k) {
+        const float *q = a.pieces + (int64_t)k * 2 * a.D + col;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] += q[e];
+      }
+      put_row<T, VEC>(dW + (int64_t)a.keys[(int64_t)(b + 1) * per_block - 1] * a.D + col, acc, a.scale);
+    }
+    for (int j = 0; j < a.G; ++j) {                      // (the same for every thread: barriers inside)
+      const int32_t bj = (int32_t)blockIdx.x * a.G + j, lj = s_last[j], pieces = lj - bj;
+      if (lj == 0 || pieces <= kLongRun) continue;
+      const int32_t share = (pieces + a.G - 1) / a.G;
+      if (on) {
+        float acc[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
+        const int32_t k0 = bj + 1 + grp * share, k1 = min(lj + 1, k0 + share);
+        for (int32_t k = k0; k < k1; ++k) {
+          const float *q = a.pieces + (int64_t)k * 2 * a.D + col;
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += q[e];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_part[threadIdx.x * VEC + e] = acc[e];
+      }
+      __syncthreads();
+      if (on && grp == 0) {
+        float acc[VEC];
+        const float *p = a.pieces + ((int64_t)bj * 2 + 1) * a.D + col;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = p[e];
+        for (int q = 0; q < a.G; ++q)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += s_part[(q * a.L + l) * VEC + e];
+        put_row<T, VEC>(dW + (int64_t)a.keys[(int64_t)(bj + 1) * per_block - 1] * a.D + col, acc, a.scale);
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------- host
+struct Layout {              // of the backward workspace, in 4-byte words
+  int32_t L, G, per_group, blocks;
+  int passes, bits;          // radix passes (0: the ids are sorted by counting) and bits of a digit
+  int32_t tile, tiles;
+  int64_t keys[2], perm[2], counts, pieces, words;
+};
+
+int lanes_of(int32_t D, int32_t dtype) {
+  const int full = dtype == RK_F32 ? 4 : 8, vec = D >= full ? full : 1;
+  return std::min(256, (D + vec - 1) / vec);
+}
+
+Layout layout_of(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
+  Layout y = {};
+  y.L = lanes_of(D, dtype);
+  y.G = 256 / y.L;
+  // 512 entries for a workgroup where there are enough of them to give every CU some, fewer otherwise
+  y.per_group = std::max(4, std::min(32, 512 / y.G));
+  while (y.per_group > 4 && rk::ceil_div(n, (int64_t)y.G * y.per_group) < 512) y.per_group /= 2;
+  y.blocks = (int32_t)rk::ceil_div(n, (int64_t)y.G * y.per_group);
+  if (n > kRankSortMax) {
+    int key_bits = 1;
+    while ((rows >> key_bits) != 0) ++key_bits;          // keys are 0 .. rows
+    y.passes = (int)rk::ceil_div(key_bits, kMaxDigitBits);
+    y.bits = (int)rk::ceil_div(key_bits, y.passes);
+    y.tile = (int32_t)std::max<int64_t>(kMinTile, rk::ceil_div(rk::ceil_div(n, kMaxTiles), kSortThreads) * kSortThreads);
+    y.tiles = (int32_t)rk::ceil_div(n, y.tile);
+  }
+  int64_t at = 0;
+  const int64_t room = rk::ceil_div(n, 4) * 4;
+  for (int k = 0; k < 2; ++k) {
+    y.keys[k] = at;
+    at += k == 0 || y.passes > 1 ? room : 0;
+    y.perm[k] = at;
+    at += k == 0 || y.passes > 1 ? room : 0;
+  }
+  y.counts = at;
+  at += (int64_t)y.tiles << y.bits;
+  y.pieces = at;
+  at += (int64_t)y.blocks * 2 * D;
+  y.words = at;
+  return y;
+}
+
+int check_common(int32_t dtype, int32_t id_bytes, int64_t n, int32_t rows, int32_t D) {
+  RK_CHECK_ARG(dtype == RK_F32 || dtype == RK_BF16 || dtype == RK_F16, "unknown element type %d", dtype);
+  RK_CHECK_ARG(id_bytes == 4 || id_bytes == 8, "ids are int32 or int64, not of %d bytes", id_bytes);
+  RK_CHECK_ARG(n >= 0 && rows >= 0 && D >= 1, "bad size: %lld ids, table %d x %d", (long long)n, rows, D);
+  RK_CHECK_ARG(n < (1ll << 31) - (1 << 24) && rows < INT32_MAX - 1, "more than 2^31 ids or rows");
+  return RK_OK;
+}
+
+template <typename T, int VEC, typename ID>
+int launch_fwd(const void *W, int64_t ldw, int32_t rows, int32_t D, const void *ids, int64_t n, float scale, void *out,
+               int32_t dtype, hipStream_t st) {
+  const int L = lanes_of(D, dtype), G = 256 / L;
+  // four rows per lane group once that still fills the GPU: their loads are in flight together
+  const int per_thread = n >= (int64_t)G * 4 * 1024 ? 4 : 1;
+  const int64_t blocks = rk::ceil_div(n, (int64_t)G * per_thread);
+  RK_CHECK_ARG(blocks < INT32_MAX, "too many ids");
+  emb_fwd_kernel<T, VEC, ID><<<(uint32_t)blocks, 256, 0, st>>>((const T *)W, ldw, rows, D, (const ID *)ids, n, scale, L,
+                                                               per_thread, (T *)out);
+  RK_CHECK_LAUNCH("emb_fwd_kernel");
+  return RK_OK;
+}
+
+template <typename SRC>
+int launch_pass(SRC src, const Layout &y, int32_t n, int pass, int32_t *ws, int to, hipStream_t st) {
+  const int shift = pass * y.bits;
+  emb_count_kernel<SRC><<<y.tiles, kSortThreads, 0, st>>>(src, n, y.tile, shift, y.bits, ws + y.counts);
+  RK_CHECK_LAUNCH("emb_count_kernel");
+  emb_place_kernel<SRC><<<y.tiles, kSortThreads, (size_t)kSortWaves * sizeof(int32_t) << y.bits, st>>>(
+      src, n, y.tile, shift, y.bits, ws + y.counts, ws + y.keys[to], ws + y.perm[to]);
+  RK_CHECK_LAUNCH("emb_place_kernel");
+  return RK_OK;
+}
+
+// the sorted keys and positions end up in buffer 0
+template <typename ID>
+int launch_sort(const ID *ids, int32_t n, int32_t rows, int64_t padding, const Layout &y, int32_t *ws, hipStream_t st) {
+  if (y.passes == 0) {
+    emb_rank_sort_kernel<ID><<<(uint32_t)rk::ceil_div(n, 32), 256, 0, st>>>(ids, n, rows, padding, ws + y.keys[0],
+                                                                           ws + y.perm[0]);
+    RK_CHECK_LAUNCH("emb_rank_sort_kernel");
+    return RK_OK;
+  }
+  for (int p = 0; p < y.passes; ++p) {
+    const int to = (y.passes - 1 - p) & 1;
+    const int rc = p == 0 ? launch_pass(FromIds<ID>{ids, rows, padding}, y, n, p, ws, to, st)
+                          : launch_pass(FromPass{ws + y.keys[to ^ 1], ws + y.perm[to ^ 1]}, y, n, p, ws, to, st);
+    if (rc) return rc;
+  }
+  return RK_OK;
+}
+
+template <typename T, int VEC>
+int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
+  const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows);
+  emb_sum_kernel<T, VEC><<<(uint32_t)blocks, 256, 0, st>>>(a, (const T *)g, (T *)dW);
+  RK_CHECK_LAUNCH("emb_sum_kernel");
+  if (a.blocks > 1) {
+    emb_join_kernel<T, VEC><<<(uint32_t)rk::ceil_div(a.blocks - 1, a.G), 256, 0, st>>>(a, (T *)dW);
+    RK_CHECK_LAUNCH("emb_join_kernel");
+  }
+  return RK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rk_embedding_fwd(const void *weight, int64_t ld_weight, int32_t rows, int32_t D, int32_t dtype, const void *ids,
+                     int32_t id_bytes, int64_t n, float scale, void *out, void *stream) {
+  if (int rc = check_common(dtype, id_bytes, n, rows, D)) return rc;
+  if (n == 0) return RK_OK;
+  RK_CHECK_ARG(ids && out && (weight || rows == 0), "null pointer");
+  RK_CHECK_ARG(ld_weight >= D || rows <= 1, "rows of the table overlap");
+  hipStream_t st = (hipStream_t)stream;
+#define RK_FWD(T, VEC)                                                                                       \
+  (id_bytes == 8 ? launch_fwd<T, VEC, int64_t>(weight, ld_weight, rows, D, ids, n, scale, out, dtype, st)    \
+                 : launch_fwd<T, VEC, int32_t>(weight, ld_weight, rows, D, ids, n, scale, out, dtype, st))
+  if (dtype == RK_F32) return D >= 4 ? RK_FWD(float, 4) : RK_FWD(float, 1);
+  if (dtype == RK_BF16) return D >= 8 ? RK_FWD(__bf16, 8) : RK_FWD(__bf16, 1);
+  return D >= 8 ? RK_FWD(_Float16, 8) : RK_FWD(_Float16, 1);
+#undef RK_FWD
+}
+
+size_t rk_embedding_bwd_ws_bytes(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
+  if (n <= 0 || rows < 0 || D < 1) return 0;
+  return (size_t)layout_of(n, rows, D, dtype).words * 4;
+}
+
+int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t id_bytes, int64_t n, int32_t rows, int32_t D,
+                     float scale, int64_t padding_idx, void *d_weight, void *ws, size_t ws_bytes, void *stream) {
+  if (int rc = check_common(dtype, id_bytes, n, rows, D)) return rc;
+  if (rows == 0) return RK_OK;
+  RK_CHECK_ARG(d_weight && (n == 0 || (grad && ids && ws)), "null pointer");
+  RK_CHECK_ARG(ws_bytes >= rk_embedding_bwd_ws_bytes(n, rows, D, dtype), "workspace too small");
+  hipStream_t st = (hipStream_t)stream;
+  int32_t *w = (int32_t *)ws;
+  const Layout y = layout_of(n, rows, D, dtype);
+  if (n > 0) {
+    const int rc = id_bytes == 8 ? launch_sort((const int64_t *)ids, (int32_t)n, rows, padding_idx, y, w, st)
+                                 : launch_sort((const int32_t *)ids, (int32_t)n, rows, padding_idx, y, w, st);
+    if (rc) return rc;
+  }
+  const SumArgs a = {w + y.keys[0], w + y.perm[0], (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks, scale,
+                     (float *)(w + y.pieces)};
+  if (dtype == RK_F32) return D >= 4 ? launch_sum<float, 4>(a, grad, d_weight, st) : launch_sum<float, 1>(a, grad, d_weight, st);
+  if (dtype == RK_BF16) return D >= 8 ? launch_sum<__bf16, 8>(a, grad, d_weight, st) : launch_sum<__bf16, 1>(a, grad, d_weight, st);
+  return D >= 8 ? launch_sum<_Float16, 8>(a, grad, d_weight, st) : launch_sum<_Float16, 1>(a, grad, d_weight, st);
+}
+
+}  // extern "C"

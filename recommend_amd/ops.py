@@ -406,6 +406,178 @@ def bpr_gather_dot_sampled(U, I, users, pos, neg_rank, pos_ptr, pos_items, mask=
 
 
 # --------------------------------------------------------------------------
+# embedding lookup with scaling; log-probabilities of item lists
+# --------------------------------------------------------------------------
+_ELEM = {torch.float32: _ffi.F32, torch.bfloat16: _ffi.BF16, torch.float16: _ffi.F16}
+
+
+def _elem(t, what):
+    code = _ELEM.get(t.dtype)
+    if code is None:
+        raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, f"{what}: float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _scratch(nbytes, device):
+    return torch.empty((nbytes + 7) // 8, dtype=torch.float64, device=device)
+
+
+def _same_device(*tensors):
+    """All of them on one HIP device (None is skipped)."""
+    _need_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+
+
+class _EmbeddingLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx):
+        out = _embedding_fwd(weight, ids, scale)
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape, scale, padding_idx)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        ids, = ctx.saved_tensors
+        (rows, D), scale, padding_idx = ctx.args
+        g = g.contiguous()
+        dw = torch.empty((rows, D), dtype=g.dtype, device=g.device)
+        kind = _ELEM[g.dtype]
+        n = ids.numel()
+        ws = _scratch(_ffi.load().rk_embedding_bwd_ws_bytes(n, rows, D, kind), g.device)
+        _ffi.call_on(g.device, "rk_embedding_bwd", ptr(g), kind, ptr(ids), ids.element_size(), n, rows, D, scale,
+                     padding_idx, ptr(dw), ptr(ws), ws.numel() * 8, stream_ptr(g.device))
+        return dw, None, None, None
+
+
+def _embedding_fwd(weight, ids, scale):
+    rows, D = weight.shape
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= D else weight.contiguous()
+    out = torch.empty((*ids.shape, D), dtype=w.dtype, device=w.device)
+    _ffi.call_on(w.device, "rk_embedding_fwd", ptr(w), w.stride(0), rows, D, _ELEM[w.dtype], ptr(ids),
+                 ids.element_size(), ids.numel(), scale, ptr(out), stream_ptr(w.device))
+    return out
+
+
+def embedding_lookup(weight, ids, scale=1.0, padding_idx=None):
+    """scale * weight[ids] with a deterministic gradient (rk_embedding_fwd / rk_embedding_bwd).
+
+    weight: [rows, D] fp32, bfloat16 or fp16; ids: int32 or int64 of any shape.  Returns [*ids.shape, D]
+    of the table's type (the product is taken in fp32 and rounded once).  The gradient of `weight` is
+    dense; contributions of equal ids are added in fp32 in the order of their positions, the same bits
+    on every run, and positions whose id is `padding_idx` (negative values count from the end, as in
+    torch.nn.Embedding) add nothing.  An id outside the table gives a row of NaN and no gradient."""
+    if weight.dim() != 2 or weight.shape[1] < 1:
+        raise ValueError(f"embedding_lookup: the table is [rows, D], got {tuple(weight.shape)}")
+    _elem(weight, "embedding_lookup")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding_lookup: ids are int32 or int64, not {ids.dtype}")
+    rows = weight.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    else:
+        if not -rows <= padding_idx < rows:
+            raise ValueError(f"embedding_lookup: padding_idx {padding_idx} outside the table of {rows} rows")
+        padding_idx = int(padding_idx) % rows
+    _same_device(weight, ids)
+    ids = ids.contiguous()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingLookup.apply(weight, ids, float(scale), padding_idx)
+    return _embedding_fwd(weight.detach(), ids, float(scale))
+
+
+PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = 0, 1, 2   # RK_PREF_* of the header
+
+
+def _list_args(scores, items, what):
+    """Checks a list operator's scores and items; returns the items as contiguous int64."""
+    _elem(scores, what)
+    if items.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: items are int32 or int64, not {items.dtype}")
+    if scores.dim() not in (2, 3) or tuple(scores.shape[:-1]) != tuple(items.shape):
+        raise ValueError(f"{what}: scores [lists, places, catalogue] and items [lists, places] (or without places), "
+                         f"got {tuple(scores.shape)} and {tuple(items.shape)}")
+    if 0 in scores.shape[1:]:
+        raise ValueError(f"{what}: no places or no catalogue in {tuple(scores.shape)}")
+    _same_device(scores, items)
+    return items.to(torch.int64).contiguous()
+
+
+def _list_geometry(scores, items):
+    """Arguments that describe scores and items to the rk_list_logps_* / rk_preference_* calls."""
+    S, V = scores.shape[0], scores.shape[-1]
+    T = scores.shape[1] if scores.dim() == 3 else 1
+    return (ptr(scores), _ELEM[scores.dtype], S, T, V, scores.stride(0), scores.stride(1) if scores.dim() == 3 else 0,
+            ptr(items), T)
+
+
+def _rows_contiguous(scores):
+    return scores if scores.stride(-1) == 1 or scores.shape[-1] == 1 else scores.contiguous()
+
+
+class _ListLogps(torch.autograd.Function):
+    """logps [S]; with ref_logps also the preference loss of the pairs (s, S/2 + s)."""
+
+    @staticmethod
+    def forward(ctx, scores, items, ref, ignore_index, average, beta, smoothing, kind):
+        scores = _rows_contiguous(scores)
+        dev, S, rows = scores.device, scores.shape[0], items.numel()
+        # (max, log sum) of every row, used places and slopes of every list: kept for the backward pass
+        keep = torch.empty(2 * rows + 2 * S, dtype=torch.float32, device=dev)
+        base = keep.data_ptr()
+        stat, used, slope = base, base + 8 * rows, base + 8 * rows + 4 * S
+        logps = torch.empty(S, dtype=torch.float32, device=dev)
+        loss = None
+        if S:
+            geo = _list_geometry(scores, items)
+            ws = _scratch(_ffi.load().rk_list_logps_ws_bytes(*geo[2:5]), dev)
+            tail = (ptr(ws), ws.numel() * 8, stream_ptr(dev))
+            if ref is None:
+                _ffi.call_on(dev, "rk_list_logps_fwd", *geo, ignore_index, average, stat, ptr(logps), used, *tail)
+            else:
+                loss = torch.empty((), dtype=torch.float32, device=dev)
+                _ffi.call_on(dev, "rk_preference_fwd", *geo, ignore_index, average, ptr(ref), beta, smoothing, kind, stat,
+                             ptr(logps), used, slope, ptr(loss), *tail)
+        ctx.save_for_backward(scores, items, keep)
+        ctx.args = (ignore_index, average, ref is not None)
+        ctx.set_materialize_grads(False)
+        return (logps,) if ref is None else (logps, loss)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logps, g_loss=None):
+        scores, items, keep = ctx.saved_tensors
+        ignore_index, average, pairs = ctx.args
+        if g_logps is None and g_loss is None:
+            return (None,) * 8
+        dev, S, rows = scores.device, scores.shape[0], items.numel()
+        g_logps = _f32c(g_logps) if g_logps is not None else None
+        g_loss = _f32c(g_loss) if g_loss is not None else None
+        dx = torch.empty(scores.shape, dtype=scores.dtype, device=dev)
+        if S:
+            base = keep.data_ptr()
+            _ffi.call_on(dev, "rk_list_logps_bwd", *_list_geometry(scores, items), ignore_index, average, base,
+                         base + 8 * rows, ptr(g_loss), base + 8 * rows + 4 * S if pairs else None, ptr(g_logps), ptr(dx),
+                         stream_ptr(dev))
+        return (dx,) + (None,) * 7
+
+
+def list_logps(scores, items, ignore_index=-100, average=False):
+    """Log-probability of every list under catalogue scores: logps[s] = sum over the places t in use of
+    (scores[s, t, items[s, t]] - logsumexp(scores[s, t, :])), divided by their number if `average`.
+
+    scores: [S, T, V] (or [S, V]) fp32, bfloat16 or fp16, rows of V contiguous, any strides between
+    them; items: [S, T] (or [S]) int32 or int64, `ignore_index` where a place is not in use (its scores are
+    not read and get a gradient of zero).  A list without places in use has 0; an item outside the
+    catalogue makes its list NaN.  Returns fp32 [S], differentiable with respect to scores."""
+    items = _list_args(scores, items, "list_logps")
+    return _ListLogps.apply(scores, items, None, int(ignore_index), int(bool(average)), 0.0, 0.0, 0)[0]
+
+
+# --------------------------------------------------------------------------
 # W2: fused node-wise layers  Y = dropout(prelu(X1 W1^T [+ X2 W2^T] + b)) [+ R]
 # --------------------------------------------------------------------------
 _seed_counter = itertools.count(1)

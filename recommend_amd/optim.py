@@ -16,6 +16,7 @@ Several GPUs: parameters listed in `sharded_params` are row shards (every rank h
 their squared gradient norms are summed over the ranks of `group` by one all-reduce of one float
 between the two launches (rk_adam_sqnorm_f32 / rk_adam_update_f32).  All other parameters are
 taken to be replicated with gradients already summed over the ranks."""
+import numpy as np
 import torch
 
 from . import _ffi
@@ -164,3 +165,212 @@ class FusedClipAdam(torch.optim.Optimizer):
         if self._dev is not None and self._lr_host != lr:
             self.lr_dev.fill_(float(lr))
             self._lr_host = lr
+
+
+_DTYPES = {torch.float32: _ffi.F32, torch.bfloat16: _ffi.BF16, torch.float16: _ffi.F16}
+_FULL = 448.0       # largest finite e4m3 value
+_TINY = 1e-30       # block maxima below this count as this
+_STATE32 = ("exp_avg", "exp_avg_sq")
+_STATE8 = ("exp_avg8", "exp_avg8_scale", "exp_avg_sq8", "exp_avg_sq8_scale")
+_TENSOR = np.dtype([("ptr", np.uint64, 6), ("n", np.int64), ("kind", np.int32, 4)])     # rk_adamw_tensor
+
+
+def encode_moment(x, keep_above_zero=False):
+    """fp32 values -> (e4m3 codes padded to whole blocks of 64, one fp32 scale per block), the form in which
+    FusedAdamW holds 8-bit moments: value = code * scale.  keep_above_zero: positive values get at least
+    the smallest code (the root of a second moment)."""
+    x = x.detach().float().reshape(-1)
+    x = torch.nn.functional.pad(x, (0, -x.numel() % _ffi.ADAMW_BLOCK)).view(-1, _ffi.ADAMW_BLOCK)
+    most = x.abs().amax(1, keepdim=True).clamp_min(_TINY)
+    y = x * (most.reciprocal() * _FULL)
+    if keep_above_zero:
+        y = torch.where(x > 0, y.clamp_min(2.0 ** -9), y)
+    return y.to(torch.float8_e4m3fn).view(-1), (most * (1.0 / _FULL)).view(-1)
+
+
+def decode_moment(code, scale, like):
+    """The fp32 values that codes and scales stand for, in the shape of the parameter `like`."""
+    return (code.float().view(-1, _ffi.ADAMW_BLOCK) * scale.unsqueeze(1)).view(-1)[:like.numel()].view(like.shape)
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (the reference trainer's other choice, train/graph_trainer.py:78-101) with
+    clip_grad_norm_ on the library's two-launch step (rk_adamw_step), over all parameter groups at once.
+
+    Parameters and gradients: contiguous fp32, bfloat16 or fp16 on one HIP device (gradients in the
+    parameter's type or fp32); the arithmetic is fp32 and a parameter is rounded once.  Up to
+    8 parameter groups with their own lr, betas, eps and weight_decay.
+
+    state_bits=32: fp32 moments, torch.optim.AdamW's state (`step`, `exp_avg`, `exp_avg_sq`).
+    state_bits=8: tensors of at least `min_8bit_size` elements hold exp_avg and the root of exp_avg_sq as
+    torch.float8_e4m3fn codes with one fp32 scale per 64 consecutive elements (`exp_avg8`,
+    `exp_avg8_scale`, `exp_avg_sq8`, `exp_avg_sq8_scale`): 2.1 bytes for each element instead of 8.
+
+    As with FusedClipAdam the step count and the learning rates live in device memory, a step can be
+    recorded in a HIP graph after one eager step, and parameters without a gradient take no part.
+    Checkpoints load across state_bits and from torch.optim.AdamW."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,
+                 state_bits=32, min_8bit_size=4096):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 8 or 32, not {state_bits}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.max_grad_norm = max_grad_norm
+        self.state_bits = state_bits
+        self.min_8bit_size = min_8bit_size
+        self._dev = None
+        self._rates = None       # learning rates that lr_dev holds
+        self._ws = None
+        self._restored_step = None
+        self.grad_norm = None    # device scalar: total gradient norm of the last clipped step, before clipping
+
+    def add_param_group(self, group):
+        if len(self.param_groups) >= _ffi.ADAMW_MAX_GROUPS:
+            raise ValueError(f"FusedAdamW takes up to {_ffi.ADAMW_MAX_GROUPS} parameter groups")
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        b1, b2 = g["betas"]
+        if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0 and g["lr"] >= 0):
+            raise ValueError("FusedAdamW: betas in [0, 1), eps, weight_decay and lr not negative")
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "_ws": None}
+
+    def _is8(self, p):
+        return self.state_bits == 8 and p.numel() >= self.min_8bit_size
+
+    def _state_for(self, p):
+        st = self.state[p]
+        if self._is8(p):
+            if "exp_avg8" not in st:
+                blocks = -(-p.numel() // _ffi.ADAMW_BLOCK)
+                for k in ("exp_avg8", "exp_avg_sq8"):
+                    st[k] = torch.zeros(blocks * _ffi.ADAMW_BLOCK, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
+                    st[k + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
+        elif "exp_avg" not in st:
+            for k in _STATE32:
+                st[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+        return st
+
+    def _init_device(self, dev):
+        self._dev = dev
+        if self._restored_step is None:
+            self._restored_step = max((int(st["step"]) for st in self.state.values() if "step" in st), default=0)
+        self.step_count = torch.full((1,), self._restored_step, dtype=torch.int64, device=dev)
+        self.lr_dev = torch.zeros(_ffi.ADAMW_MAX_GROUPS, dtype=torch.float32, device=dev)
+        self.grad_norm = torch.zeros(1, dtype=torch.float32, device=dev)
+
+    def _check(self, p, g):
+        if not (p.is_cuda and p.dtype in _DTYPES and p.is_contiguous() and g.layout == torch.strided and g.is_contiguous()
+                and (g.dtype == p.dtype or g.dtype == torch.float32)):
+            raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, "FusedAdamW: contiguous fp32, bfloat16 or fp16 parameters on a HIP "
+                               "device with dense gradients of their type or fp32 only")
+        if p.device != self._dev or g.device != self._dev:
+            raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, f"FusedAdamW: all parameters on one device ({self._dev})")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        rows, kinds, sizes, dev = [], [], [], self._dev
+        for k, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                g = p.grad
+                if g is None or not p.numel():
+                    continue
+                if dev is None:
+                    if not p.is_cuda:
+                        raise _ffi.RkError(_ffi.RK_ERR_NODEV, "FusedAdamW: parameters on a HIP device only")
+                    self._init_device(p.device)
+                    dev = self._dev
+                self._check(p, g)
+                st = self._state_for(p)
+                a, b = (st[x].data_ptr() for x in (_STATE8[::2] if "exp_avg8" in st else _STATE32))
+                sa, sb = (st[x].data_ptr() for x in _STATE8[1::2]) if "exp_avg8" in st else (0, 0)
+                rows.append((p.data_ptr(), g.data_ptr(), a, b, sa, sb))
+                sizes.append(p.numel())
+                kinds.append((_DTYPES[p.dtype], _DTYPES[g.dtype], k, 0))
+        if not rows:
+            return loss
+        n = len(rows)
+        table = np.empty(n, _TENSOR)
+        table["ptr"], table["n"], table["kind"] = rows, sizes, kinds
+        groups = (_ffi.AdamwGroup * len(self.param_groups))()
+        for dst, group in zip(groups, self.param_groups):
+            (dst.beta1, dst.beta2), dst.eps, dst.weight_decay = group["betas"], group["eps"], group["weight_decay"]
+        self.sync_lr()
+        need = _ffi.load().rk_adamw_ws_bytes(n)
+        if self._ws is None or self._ws.numel() * 8 < need:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
+            self._ws = torch.zeros(need // 8, dtype=torch.float64, device=dev)
+        _ffi.call_on(dev, "rk_adamw_step", ptr(table), n, groups, len(groups), ptr(self.step_count), ptr(self.lr_dev),
+                     float(self.max_grad_norm or 0.0), ptr(self.grad_norm), ptr(self._ws), self._ws.numel() * 8,
+                     stream_ptr(dev))
+        return loss
+
+    def sync_lr(self):
+        """Push learning rates changed by a scheduler to device memory (step() does it; call it for a step that
+        is replayed from a graph, outside the capture)."""
+        rates = [float(g["lr"]) for g in self.param_groups]
+        if self._dev is None or rates == self._rates:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            if self._rates is None:
+                raise RuntimeError("run one optimizer step before capturing it in a graph")
+            return
+        for k, rate in enumerate(rates):
+            if self._rates is None or k >= len(self._rates) or self._rates[k] != rate:
+                self.lr_dev[k].fill_(rate)
+        self._rates = rates
+
+    def state_dict(self):
+        """torch.optim.AdamW's layout (and the keys of 8-bit moments): every parameter's state carries `step`
+        beside its moments (reading the device counter synchronises)."""
+        if self._dev is not None:
+            t = float(self.step_count.item())
+            for st in self.state.values():
+                if st:
+                    st["step"] = torch.tensor(t)
+        return super().state_dict()
+
+    def load_state_dict(self, state_dict):
+        """Moments and step count of a checkpoint: this optimizer's with either number of bits, or
+        torch.optim.AdamW's.  Moments are converted to the form this optimizer holds.  Buffers that exist
+        keep their memory and take the checkpoint's values, so a step recorded in a HIP graph before the
+        load goes on with them.  Call it outside graph capture."""
+        old = {p: dict(st) for p, st in self.state.items()}
+        saved = state_dict["state"]
+        order = [i for g in state_dict["param_groups"] for i in g["params"]]
+        super().load_state_dict(state_dict)
+        # (torch casts floating state to the parameter's type on the way: the values are taken from the
+        # checkpoint itself)
+        for i, p in zip(order, [p for g in self.param_groups for p in g["params"]]):
+            src = saved.get(i)
+            if not src or not ("exp_avg" in src or "exp_avg8" in src):
+                continue
+            src = {k: v.to(p.device) if torch.is_tensor(v) else v for k, v in src.items()}
+            st = {"step": torch.tensor(float(src.get("step", 0)))}
+            if self._is8(p) and "exp_avg8" in src:
+                st.update({k: src[k].clone() for k in _STATE8})
+            elif self._is8(p):
+                st["exp_avg8"], st["exp_avg8_scale"] = encode_moment(src["exp_avg"])
+                st["exp_avg_sq8"], st["exp_avg_sq8_scale"] = encode_moment(src["exp_avg_sq"].float().sqrt(), True)
+            elif "exp_avg" in src:
+                st.update({k: src[k].detach().float().reshape(p.shape).clone() for k in _STATE32})
+            else:
+                st["exp_avg"] = decode_moment(src["exp_avg8"], src["exp_avg8_scale"], p)
+                st["exp_avg_sq"] = decode_moment(src["exp_avg_sq8"], src["exp_avg_sq8_scale"], p).square()
+            for k, v in st.items():
+                have = old.get(p, {}).get(k)
+                if k != "step" and have is not None and have.shape == v.shape and have.dtype == v.dtype:
+                    have.copy_(v)
+                    st[k] = have
+            self.state[p] = st
+        self._restored_step = max((int(st["step"]) for st in self.state.values() if "step" in st), default=0)
+        if self._dev is not None:
+            self.step_count.fill_(self._restored_step)
+            self._rates = None
+            self.sync_lr()

@@ -1,0 +1,168 @@
+"""What the embedding, list and AdamW operators refuse, before anything reaches a device: wrong types,
+shapes and constants in the Python entry points, wrong sizes and pointers in the C ABI."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from recommend_amd import _ffi, ops
+from recommend_amd.loss import list_logps, preference_loss
+from recommend_amd.optim import FusedAdamW, decode_moment, encode_moment
+
+F = torch.zeros
+
+
+def long(*s):
+    return torch.zeros(s, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("weight,ids,kw,error", [
+    (F(4), long(2), {}, "table is"),
+    (F(4, 0), long(2), {}, "table is"),
+    (F(4, 3).double(), long(2), {}, "float32, bfloat16 or float16"),
+    (F(4, 3), F(2), {}, "int32 or int64"),
+    (F(4, 3), long(2).to(torch.int16), {}, "int32 or int64"),
+    (F(4, 3), long(2), {"padding_idx": 4}, "outside the table"),
+    (F(4, 3), long(2), {"padding_idx": -5}, "outside the table"),
+    (F(4, 3), long(2), {}, "HIP device"),
+])
+def test_embedding_lookup_refuses(weight, ids, kw, error):
+    with pytest.raises((ValueError, _ffi.RkError), match=error):
+        ops.embedding_lookup(weight, ids, **kw)
+
+
+@pytest.mark.parametrize("scores,items,error", [
+    (F(4, 3, 5), long(4), "lists, places, catalogue"),
+    (F(4, 3, 5), long(4, 2), "lists, places, catalogue"),
+    (F(5), long(), "lists, places, catalogue"),
+    (F(4, 0, 5), long(4, 0), "no places"),
+    (F(4, 3, 0), long(4, 3), "no places"),
+    (F(4, 3, 5).double(), long(4, 3), "float32, bfloat16 or float16"),
+    (F(4, 3, 5), F(4, 3), "int32 or int64"),
+    (F(4, 3, 5), long(4, 3), "HIP device"),
+])
+def test_list_logps_refuses(scores, items, error):
+    with pytest.raises((ValueError, _ffi.RkError), match=error):
+        list_logps(scores, items)
+
+
+@pytest.mark.parametrize("lists,ref,kw,error", [
+    (3, 3, {}, "pairs of lists"),
+    (0, 0, {}, "pairs of lists"),
+    (4, 2, {}, "reference log-probability"),
+    (4, 4, {"beta": 0.0}, "beta"),
+    (4, 4, {"beta": float("nan")}, "beta"),
+    (4, 4, {"label_smoothing": 1.5}, "label_smoothing"),
+    (4, 4, {"label_smoothing": 0.1, "kind": "hinge"}, "sigmoid form only"),
+    (4, 4, {"kind": "ranked"}, "kind is one of"),
+    (4, 4, {}, "HIP device"),
+])
+def test_preference_loss_refuses(lists, ref, kw, error):
+    with pytest.raises((ValueError, _ffi.RkError), match=error):
+        preference_loss(F(lists, 3, 5), long(lists, 3), F(ref), **kw)
+
+
+def test_adamw_refuses():
+    p = lambda: torch.nn.Parameter(F(4))  # noqa: E731
+    with pytest.raises(ValueError, match="state_bits"):
+        FusedAdamW([p()], state_bits=4)
+    with pytest.raises(ValueError, match="betas"):
+        FusedAdamW([p()], betas=(0.9, 1.0))
+    with pytest.raises(ValueError, match="betas"):
+        FusedAdamW([p()], weight_decay=-0.1)
+    with pytest.raises(ValueError, match="up to 8"):
+        FusedAdamW([{"params": [p()]} for _ in range(9)])
+    opt = FusedAdamW([p()])
+    opt.step()                                            # no gradient: nothing to do
+    opt.param_groups[0]["params"][0].grad = F(4)
+    with pytest.raises(_ffi.RkError, match="HIP device"):
+        opt.step()
+
+
+def refused(name, *args, error=""):
+    assert getattr(_ffi.load(), name)(*args) == _ffi.RK_ERR_ARG
+    assert error in _ffi.last_error(), _ffi.last_error()
+
+
+def test_c_abi_refuses_bad_embedding_calls():
+    b = _ffi.ptr(np.zeros(64, np.float64))
+    fwd = lambda dtype=0, bytes_=8, n=2, rows=4, D=4, ld=4, w=b, ids=b: (w, ld, rows, D, dtype, ids, bytes_, n, 1.0, b, None)  # noqa: E731,E501
+    for kw, error in (({"dtype": 3}, "element type"), ({"bytes_": 2}, "int32 or int64"), ({"n": -1}, "bad size"),
+                      ({"D": 0}, "bad size"), ({"rows": -1}, "bad size"), ({"ld": 3}, "overlap"), ({"w": None}, "null"),
+                      ({"ids": None}, "null"), ({"n": 1 << 31}, "2^31")):
+        refused("rk_embedding_fwd", *fwd(**kw), error=error)
+    assert _ffi.load().rk_embedding_fwd(*fwd(n=0)) == _ffi.RK_OK
+    need = _ffi.load().rk_embedding_bwd_ws_bytes(2, 4, 4, 0)
+    assert need > 0
+    bwd = lambda dtype=0, bytes_=8, n=2, g=b, dw=b, ws=b, room=need: (g, dtype, b, bytes_, n, 4, 4, 1.0, -1, dw, ws, room, None)  # noqa: E731,E501
+    for kw, error in (({"dtype": -1}, "element type"), ({"bytes_": 1}, "int32 or int64"), ({"g": None}, "null"),
+                      ({"dw": None}, "null"), ({"ws": None}, "null"), ({"room": need - 1}, "workspace")):
+        refused("rk_embedding_bwd", *bwd(**kw), error=error)
+
+
+def test_c_abi_refuses_bad_list_calls():
+    b, lib = _ffi.ptr(np.zeros(4096, np.float64)), _ffi.load()
+    need = lib.rk_list_logps_ws_bytes(4, 3, 5)
+    geo = lambda dtype=0, S=4, T=3, V=5, x=b, items=b: (x, dtype, S, T, V, T * V, V, items, T, -100, 0)  # noqa: E731
+    for kw, error in (({"dtype": 9}, "element type"), ({"S": -1}, "bad size"), ({"V": 0}, "bad size"),
+                      ({"V": 1 << 30}, "2^30"), ({"x": None}, "null"), ({"items": None}, "null")):
+        refused("rk_list_logps_fwd", *geo(**kw), b, b, b, b, need, None, error=error)
+        refused("rk_list_logps_bwd", *geo(**kw), b, b, b, b, b, b, None, error=error)
+    refused("rk_list_logps_fwd", *geo(T=0), b, b, b, b, need, None, error="without places")
+    refused("rk_list_logps_fwd", *geo(), b, b, b, b, need - 1, None, error="workspace")
+    refused("rk_list_logps_bwd", *geo(), b, b, b, None, b, b, None, error="slopes")
+    pref = lambda beta=0.1, eps=0.0, kind=0, ref=b, room=need, **kw: (  # noqa: E731
+        *geo(**kw), ref, beta, eps, kind, b, b, b, b, b, b, room, None)
+    for kw, error in (({"S": 3}, "pairs"), ({"S": 0}, "pairs"), ({"T": 0}, "pairs"), ({"beta": 0.0}, "beta"),
+                      ({"eps": -0.1}, "smoothing"), ({"eps": 0.1, "kind": 1}, "sigmoid form"), ({"kind": 3}, "kind"),
+                      ({"ref": None}, "null"), ({"room": 8}, "workspace")):
+        refused("rk_preference_fwd", *pref(**kw), error=error)
+
+
+def test_c_abi_refuses_bad_adamw_calls():
+    buf = np.zeros(8192, np.float64)
+    b, at = _ffi.ptr(buf), buf.ctypes.data
+    at += -at % 16
+    need = _ffi.load().rk_adamw_ws_bytes(1)
+
+    def call(error, group=None, n_groups=1, ws=at, room=need, **kw):
+        f = dict(param=at, grad=at, exp_avg=at, exp_avg_sq=at, n=8)
+        f.update(kw)
+        t = _ffi.AdamwTensor(**f)
+        g = _ffi.AdamwGroup(*(group or (0.9, 0.999, 1e-8, 0.0)))
+        refused("rk_adamw_step", ctypes.byref(t), 1, ctypes.byref(g), n_groups, b, b, 0.0, None, ws, room, None, error=error)
+
+    call("null", n=0)
+    call("null", grad=None)
+    call("scales", exp_avg_scale=at)
+    call("element type", param_dtype=5)
+    call("parameter's type", grad_dtype=1)
+    call("bad AdamW constants", group=(1.0, 0.999, 1e-8, 0.0))
+    call("bad AdamW constants", group=(0.9, 0.999, -1e-8, 0.0))
+    call("parameter groups", n_groups=9)
+    call("parameter groups", n_groups=0)
+    call("workspace", room=need - 1)
+    call("workspace", ws=at + 8)
+    call("4-byte aligned", exp_avg=at + 2, exp_avg_scale=at, exp_avg_sq_scale=at)
+    assert _ffi.load().rk_adamw_step(None, 0, None, 0, None, None, 0.0, None, None, 0, None) == _ffi.RK_OK
+    assert ctypes.sizeof(_ffi.AdamwTensor) == 72 and ctypes.sizeof(_ffi.AdamwGroup) == 32
+
+
+@pytest.mark.parametrize("n", [1, 63, 64, 65, 1000])
+def test_moments_survive_encoding(n):
+    """value = code * scale: e4m3 keeps four significant bits (half a step is 2^-4 of the value) down to 2^-6 of
+    scale, and half of 2^-9 of scale below; scale and product round twice more in fp32."""
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g))
+    code, scale = encode_moment(x)
+    assert code.numel() == scale.numel() * 64 and code.dtype == torch.float8_e4m3fn
+    back = decode_moment(code, scale, x)
+    each = scale.repeat_interleave(64)[:n]
+    tol = torch.maximum(x.abs() * 2.0 ** -4, each * 2.0 ** -10) * (1 + 2.0 ** -20)
+    assert bool(((back - x).abs() <= tol).all())
+    assert bool((code.float()[n:] == 0).all())
+    assert torch.equal(*(encode_moment(decode_moment(code, scale, x))[0].view(torch.uint8)[:n], code.view(torch.uint8)[:n]))
+    tiny = torch.tensor([1.0, 1e-12, 0.0])
+    code, scale = encode_moment(tiny, keep_above_zero=True)
+    assert code.view(torch.uint8)[:3].tolist() == [0x7E, 1, 0]
