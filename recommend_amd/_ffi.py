@@ -232,14 +232,24 @@ def ptr(t):
     return c_void_p(t.ctypes.data)
 
 
+_functions = {}
+
+
 def call_on(device, name, *args):
-    """`call` with `device` current: a launch goes to the device its stream belongs to."""
+    """`call` with `device` current (a launch goes to the device its stream belongs to) and that device's
+    current stream as the last argument."""
     import torch
-    if torch.cuda.current_device() == device.index:
-        call(name, *args)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args)
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != RK_OK:
+        check(code)
 
 
 def stream_ptr(device=None):

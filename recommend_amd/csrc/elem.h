@@ -5,6 +5,7 @@
 
 namespace rk {
 
+typedef uint32_t u32x4_at_elem __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2v __attribute__((ext_vector_type(2)));
@@ -59,6 +60,24 @@ struct Pack {
   uint32_t w[kWords];
   __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(w, p, kBytes); }
   __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, w, kBytes); }
+  // the same for data that is touched once: it does not push other data out of the caches
+  __device__ __forceinline__ void load_once(const T *p) {
+    if constexpr (kWords == 4) {
+      const u32x4_at_elem v = __builtin_nontemporal_load((const u32x4_at_elem *)p);
+      __builtin_memcpy(w, &v, 16);
+    } else {
+      load(p);
+    }
+  }
+  __device__ __forceinline__ void store_once(T *p) const {
+    if constexpr (kWords == 4) {
+      u32x4_at_elem v;
+      __builtin_memcpy(&v, w, 16);
+      __builtin_nontemporal_store(v, (u32x4_at_elem *)p);
+    } else {
+      store(p);
+    }
+  }
   __device__ __forceinline__ void widen(float (&o)[N]) const {
     if constexpr (kBytes < 4) {
       T x;

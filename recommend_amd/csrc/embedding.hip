@@ -7,8 +7,8 @@
 // whatever the tensors' type, the same bits on every run, and rounded once.
 //
 // Sort: up to kRankSortMax ids one launch counts, for every id, the ids that come before it.  More
-// ids take an LSD radix sort with digits of up to 9 bits: per digit one launch that counts a tile's
-// digits and one that places them (every workgroup adds up the counts in front of its own itself).
+// ids take an LSD radix sort with digits of up to 9 bits: per digit one launch that counts every
+// tile's digits, one that adds up each digit's counts over the tiles and one that places the ids.
 // Padded and out-of-range ids get the key `rows`: they come last and add nothing.
 //
 // Sum: a lane group takes `per_group` consecutive sorted entries and keeps the running row in
@@ -22,15 +22,19 @@
 
 namespace {
 
-constexpr int kRankSortMax = 4096;    // ids sorted by counting
-constexpr int kSortThreads = 1024;
+constexpr int kRankSortMax = 8192;    // ids sorted by counting
+constexpr int kRankThreads = 16;      // threads that count for one id
+constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / rk::kWave;
-constexpr int kMaxDigitBits = 9;
-constexpr int kMaxTiles = 128;        // tiles of a radix pass: every workgroup adds up this many counts per digit
-constexpr int kMinTile = 8192;
+constexpr int kMaxDigitBits = 9;      // one thread for each digit
+constexpr int kTileSteps = 8;         // ids of a thread: they stay in registers
+constexpr int kTile = kSortThreads * kTileSteps;
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
 constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
-constexpr int kLongRun = 32;          // workgroup pieces of a row above which a whole workgroup joins them
+constexpr int kPerGroup = 16;         // sorted entries of a lane group
+constexpr int kJoins = 16;            // workgroup borders that one workgroup of the closing launch looks at
+constexpr int64_t kStreamBytes = 64 << 20;   // looked-up rows from this size on are stored past the caches
+constexpr int kLongRun = 8;          // workgroup pieces of a row above which a whole workgroup joins them
 
 // the sort key of an id: ids outside [0, rows) and the padding id go behind all rows
 template <typename ID>
@@ -39,63 +43,72 @@ __device__ __forceinline__ int32_t key_of(ID id, int32_t rows, int64_t padding) 
 }
 
 // ------------------------------------------------------------------------------------- lookup
-template <typename T, int VEC, typename ID>
+// ROWS rows of a lane group are in flight together.  ONCE: the output is larger than what the caches
+// should hold and is stored past them; the table's rows stay cached (2^20 rows of 256 bytes from a
+// table of 65 MB: 69 us instead of 81, and 20 us less for the launch that follows).
+template <typename T, int VEC, typename ID, int ROWS, bool ONCE>
 __global__ __launch_bounds__(256) void emb_fwd_kernel(const T *__restrict__ W, int64_t ldw, int32_t rows, int32_t D,
                                                       const ID *__restrict__ ids, int64_t n, float scale, int32_t L,
-                                                      int32_t per_thread, T *__restrict__ out) {
+                                                      T *__restrict__ out) {
   const int G = 256 / L, grp = threadIdx.x / L, l = threadIdx.x - grp * L;
   if (grp >= G) return;
-  const int64_t base = (int64_t)blockIdx.x * G * per_thread;
-  for (int c0 = 0; c0 < D; c0 += L * VEC) {
-    if (c0 + l * VEC >= D) break;
-    const int col = min(c0 + l * VEC, D - VEC);   // the last vector of a row overlaps the one before it
-    for (int r0 = 0; r0 < per_thread; r0 += 4) {
-      rk::Pack<T, VEC> v[4];
-      bool ok[4];
+  const int64_t i0 = (int64_t)blockIdx.x * G * ROWS + grp;
+  int64_t at[ROWS];
+  bool ok[ROWS];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t i = base + (int64_t)(r0 + j) * G + grp;
-        const ID id = r0 + j < per_thread && i < n ? ids[i] : (ID)-1;
-        ok[j] = id >= 0 && (int64_t)id < rows;
-        if (ok[j]) v[j].load(W + (int64_t)id * ldw + col);
-      }
+  for (int j = 0; j < ROWS; ++j) {
+    const ID id = ids[min(i0 + (int64_t)j * G, n - 1)];
+    ok[j] = id >= 0 && (int64_t)id < rows;
+    at[j] = ok[j] ? (int64_t)id * ldw : 0;
+  }
+  for (int c0 = l * VEC; c0 < D; c0 += L * VEC) {
+    const int col = min(c0, D - VEC);   // the last vector of a row overlaps the one before it
+    rk::Pack<T, VEC> v[ROWS];
+    if (rows > 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t i = base + (int64_t)(r0 + j) * G + grp;
-        if (r0 + j >= per_thread || i >= n) continue;
-        float x[VEC];
-        if (ok[j]) {
-          v[j].widen(x);
+      for (int j = 0; j < ROWS; ++j) v[j].load(W + at[j] + col);
+    }
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) x[e] *= scale;
-        } else {
+    for (int j = 0; j < ROWS; ++j) {
+      const int64_t i = i0 + (int64_t)j * G;
+      float x[VEC];
+      v[j].widen(x);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) x[e] = __builtin_nanf("");   // no row has this id
-        }
-        v[j].narrow(x);
-        v[j].store(out + i * D + col);
+      for (int e = 0; e < VEC; ++e) x[e] = ok[j] ? x[e] * scale : __builtin_nanf("");   // NaN: no row has this id
+      v[j].narrow(x);
+      if (i < n) {
+        if constexpr (ONCE)
+          v[j].store_once(out + i * D + col);
+        else
+          v[j].store(out + i * D + col);
       }
     }
   }
 }
 
 // --------------------------------------------------------------------------------------- sort
-// position of id i = number of ids in front of it: smaller keys, and equal keys at lower positions.
-// 32 ids per workgroup, eight threads each.
+// position of id i = number of ids in front of it: smaller keys, and equal keys at lower positions
 template <typename ID>
 __global__ __launch_bounds__(256) void emb_rank_sort_kernel(const ID *__restrict__ ids, int32_t n, int32_t rows,
                                                             int64_t padding, int32_t *__restrict__ keys,
                                                             int32_t *__restrict__ perm) {
   __shared__ int32_t s_key[kRankSortMax];
-  for (int j = threadIdx.x; j < n; j += 256) s_key[j] = key_of(ids[j], rows, padding);
+  const int32_t room = (n + 3) / 4 * 4;
+  for (int j = threadIdx.x; j < room; j += 256) s_key[j] = j < n ? key_of(ids[j], rows, padding) : INT32_MAX;
   __syncthreads();
-  const int i = blockIdx.x * 32 + threadIdx.x / 8, sub = threadIdx.x % 8;
+  const int i = blockIdx.x * (256 / kRankThreads) + threadIdx.x / kRankThreads, sub = threadIdx.x % kRankThreads;
   const int32_t my = i < n ? s_key[i] : 0;
   int before = 0;
-  if (i < n)
-    for (int j = sub; j < n; j += 8) before += s_key[j] < my + (j < i ? 1 : 0);
+#pragma unroll 4
+  for (int j = sub * 4; j < room; j += kRankThreads * 4) {
+    const int4 k = *reinterpret_cast<const int4 *>(&s_key[j]);
+    before += k.x < my + (j < i ? 1 : 0);
+    before += k.y < my + (j + 1 < i ? 1 : 0);
+    before += k.z < my + (j + 2 < i ? 1 : 0);
+    before += k.w < my + (j + 3 < i ? 1 : 0);
+  }
 #pragma unroll
-  for (int off = 4; off > 0; off >>= 1) before += __shfl_xor(before, off, 8);
+  for (int off = kRankThreads / 2; off > 0; off >>= 1) before += __shfl_xor(before, off, kRankThreads);
   if (i < n && sub == 0) {
     keys[before] = my;
     perm[before] = i;
@@ -118,54 +131,50 @@ struct FromPass {
 };
 
 template <typename SRC>
-__global__ __launch_bounds__(kSortThreads) void emb_count_kernel(SRC src, int32_t n, int32_t tile, int shift, int bits,
+__global__ __launch_bounds__(kSortThreads) void emb_count_kernel(SRC src, int32_t n, int shift, int bits,
                                                                  int32_t *__restrict__ counts) {
   __shared__ int32_t s_count[1 << kMaxDigitBits];
   const int nd = 1 << bits;
-  for (int d = threadIdx.x; d < nd; d += kSortThreads) s_count[d] = 0;
+  if ((int)threadIdx.x < nd) s_count[threadIdx.x] = 0;
+  int32_t key[kTileSteps];
+  const int64_t lo = (int64_t)blockIdx.x * kTile + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) key[k] = lo + k * kSortThreads < n ? src.key((int32_t)(lo + k * kSortThreads)) : -1;
   __syncthreads();
-  const int32_t lo = (int32_t)blockIdx.x * tile, hi = (int32_t)min((int64_t)n, (int64_t)lo + tile);
-  for (int32_t i = lo + threadIdx.x; i < hi; i += kSortThreads)
-    atomicAdd(&s_count[(src.key(i) >> shift) & (nd - 1)], 1);
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k)
+    if (key[k] >= 0) atomicAdd(&s_count[(key[k] >> shift) & (nd - 1)], 1);
   __syncthreads();
-  for (int d = threadIdx.x; d < nd; d += kSortThreads) counts[(int64_t)blockIdx.x * nd + d] = s_count[d];
+  if ((int)threadIdx.x < nd) counts[(int64_t)blockIdx.x * nd + threadIdx.x] = s_count[threadIdx.x];
 }
 
-// Places one tile: every wavefront owns a consecutive part of it, so that (wavefront, step, lane) is the
-// order of the positions and equal digits keep it.
-template <typename SRC>
-__global__ __launch_bounds__(kSortThreads) void emb_place_kernel(SRC src, int32_t n, int32_t tile, int shift, int bits,
-                                                                 const int32_t *__restrict__ counts,
-                                                                 int32_t *__restrict__ keys, int32_t *__restrict__ perm) {
-  extern __shared__ int32_t s_off[];   // [kSortWaves][nd]: next place of a digit for every wavefront
-  __shared__ int32_t s_total[1 << kMaxDigitBits], s_front[1 << kMaxDigitBits], s_wave[kSortWaves];
-  const int nd = 1 << bits, t = threadIdx.x, wave = t / rk::kWave, lane = t % rk::kWave;
-  for (int i = t; i < kSortWaves * nd; i += kSortThreads) s_off[i] = 0;
-  for (int d = t; d < nd; d += kSortThreads) s_total[d] = s_front[d] = 0;
+// exclusive sums of every digit's counts over the tiles, in place, and the digits' totals.  16 digits per
+// workgroup (64 bytes of a tile's counts), 16 threads each, which take consecutive shares of the tiles.
+__global__ __launch_bounds__(256) void emb_scan_kernel(int32_t *__restrict__ counts, int32_t tiles, int nd,
+                                                       int32_t *__restrict__ totals) {
+  __shared__ int32_t s_sum[16][16];
+  const int q = threadIdx.x / 16, dl = threadIdx.x % 16, d = (int)blockIdx.x * 16 + dl;
+  const int32_t share = (tiles + 15) / 16, t0 = min(tiles, q * share), t1 = d < nd ? min(tiles, t0 + share) : t0;
+  int32_t sum = 0;
+#pragma unroll 8
+  for (int32_t t = t0; t < t1; ++t) sum += counts[(int64_t)t * nd + d];
+  s_sum[q][dl] = sum;
   __syncthreads();
-  // counts of every digit over all tiles and over the tiles in front of this one (integer sums: any order)
-  const int my_tile = blockIdx.x, n_tiles = gridDim.x, parts = kSortThreads / nd;
-  {
-    const int d = t & (nd - 1), part = t / nd;
-    int32_t total = 0, front = 0;
-    for (int k = part; k < n_tiles; k += parts) {
-      const int32_t c = counts[(int64_t)k * nd + d];
-      total += c;
-      front += k < my_tile ? c : 0;
-    }
-    atomicAdd(&s_total[d], total);
-    atomicAdd(&s_front[d], front);
+  int32_t at = 0;
+  for (int k = 0; k < q; ++k) at += s_sum[k][dl];
+#pragma unroll 8
+  for (int32_t t = t0; t < t1; ++t) {
+    const int32_t c = counts[(int64_t)t * nd + d];
+    counts[(int64_t)t * nd + d] = at;
+    at += c;
   }
-  // digits of every wavefront's part of the tile
-  const int32_t part_len = tile / kSortWaves;
-  const int64_t end = min((int64_t)n, (int64_t)my_tile * tile + tile);
-  const int64_t lo = (int64_t)my_tile * tile + (int64_t)wave * part_len;
-  const int64_t hi = min(end, lo + part_len);
-  for (int64_t i = lo + lane; i < hi; i += rk::kWave)
-    atomicAdd(&s_off[wave * nd + ((src.key((int32_t)i) >> shift) & (nd - 1))], 1);
-  __syncthreads();
-  // exclusive sum over the digits (nd <= kSortThreads), then over the wavefronts of this tile
-  int32_t total = t < nd ? s_total[t] : 0, incl = total;
+  if (q == 15 && d < nd) totals[d] = at;
+}
+
+// exclusive sum over the threads of a sorting workgroup (s_wave: kSortWaves words of scratch)
+__device__ __forceinline__ int32_t block_scan(int32_t v, int32_t *s_wave) {
+  const int lane = threadIdx.x % rk::kWave, wave = threadIdx.x / rk::kWave;
+  int32_t incl = v;
 #pragma unroll
   for (int off = 1; off < rk::kWave; off <<= 1) {
     const int32_t o = __shfl_up(incl, off, rk::kWave);
@@ -173,9 +182,47 @@ __global__ __launch_bounds__(kSortThreads) void emb_place_kernel(SRC src, int32_
   }
   if (lane == rk::kWave - 1) s_wave[wave] = incl;
   __syncthreads();
+  int32_t at = incl - v;
+  for (int w = 0; w < wave; ++w) at += s_wave[w];
+  return at;
+}
+
+// Places one tile.  Every wavefront owns a consecutive part of it, so that (wavefront, step, lane) is the
+// order of the positions and equal digits keep it.  The tile is put in order in LDS first and then
+// written from there: ids of one digit go to consecutive places (written straight from the
+// registers, 4-byte stores all over the output, this launch took 20 us for 2^20 ids instead of 14).
+template <typename SRC>
+__global__ __launch_bounds__(kSortThreads) void emb_place_kernel(SRC src, int32_t n, int shift, int bits,
+                                                                 const int32_t *__restrict__ counts,
+                                                                 const int32_t *__restrict__ totals,
+                                                                 int32_t *__restrict__ keys, int32_t *__restrict__ perm) {
+  __shared__ int32_t s_off[kSortWaves << kMaxDigitBits];   // [wavefront][digit]: next place in the tile
+  __shared__ int32_t s_to[1 << kMaxDigitBits];             // place in the output minus place in the tile
+  __shared__ int32_t s_key[kTile], s_pos[kTile];
+  __shared__ int32_t s_wave[2][kSortWaves];
+  const int nd = 1 << bits, t = threadIdx.x, wave = t / rk::kWave, lane = t % rk::kWave;
+  const int64_t tile0 = (int64_t)blockIdx.x * kTile, lo = tile0 + wave * (rk::kWave * kTileSteps) + lane;
+  int32_t key[kTileSteps], pos[kTileSteps];
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const bool in = lo + k * rk::kWave < n;
+    key[k] = in ? src.key((int32_t)(lo + k * rk::kWave)) : -1;
+    pos[k] = in ? src.pos((int32_t)(lo + k * rk::kWave)) : 0;
+  }
+  const int32_t total = t < nd ? totals[t] : 0, front = t < nd ? counts[(int64_t)blockIdx.x * nd + t] : 0;
+  for (int i = t; i < kSortWaves * nd; i += kSortThreads) s_off[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k)
+    if (key[k] >= 0) atomicAdd(&s_off[wave * nd + ((key[k] >> shift) & (nd - 1))], 1);
+  const int32_t out0 = block_scan(total, s_wave[0]) + front;   // (its barrier also closes the counting)
+  int32_t mine = 0;
+  if (t < nd)
+    for (int w = 0; w < kSortWaves; ++w) mine += s_off[w * nd + t];
+  int32_t at = block_scan(mine, s_wave[1]);
   if (t < nd) {
-    int32_t at = incl - total + s_front[t];
-    for (int w = 0; w < wave; ++w) at += s_wave[w];
+    s_to[t] = out0 - at;
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
       const int32_t c = s_off[w * nd + t];
       s_off[w * nd + t] = at;
@@ -183,30 +230,49 @@ __global__ __launch_bounds__(kSortThreads) void emb_place_kernel(SRC src, int32_
     }
   }
   __syncthreads();
-  for (int64_t i0 = lo; i0 < hi; i0 += rk::kWave) {
-    const int64_t i = i0 + lane;
-    const bool in = i < hi;
-    const int32_t key = in ? src.key((int32_t)i) : 0, pos = in ? src.pos((int32_t)i) : 0;
-    const int d = (key >> shift) & (nd - 1);
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((d >> b) & 1);
-      same &= (d >> b) & 1 ? set : ~set;
+  // rank of a lane among the lanes of its digit, their number and whether it is the last of them: these do
+  // not wait for each other, the eight LDS steps below do
+  int rank[kTileSteps], same_n[kTileSteps];
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const int d = (key[k] >> shift) & (nd - 1);
+    uint64_t same = __ballot(key[k] >= 0);
+#pragma unroll
+    for (int b = 0; b < kMaxDigitBits; ++b) {            // (bits that a digit does not have are zero in all lanes)
+      const bool one = (d >> b) & 1;
+      const uint64_t set = __ballot(one);
+      same &= one ? set : ~set;
     }
-    if (in) {
-      const int rank = __popcll(same & ((1ull << lane) - 1));
-      const int32_t at = s_off[wave * nd + d] + rank;
-      keys[at] = key;
-      perm[at] = pos;
+    rank[k] = __popcll(same & ((1ull << lane) - 1));
+    same_n[k] = (same >> lane) == 1 ? __popcll(same) : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    int32_t *off = &s_off[wave * nd + ((key[k] >> shift) & (nd - 1))];
+    int32_t first = 0;
+    if (key[k] >= 0) {
+      first = *off;
+      s_key[first + rank[k]] = key[k];
+      s_pos[first + rank[k]] = pos[k];
     }
     // (a wavefront's LDS operations complete in program order: all lanes have read before one writes)
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (in && (same >> lane) == 1) s_off[wave * nd + d] += __popcll(same);   // the last lane with this digit
+    if (key[k] >= 0 && same_n[k]) *off = first + same_n[k];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  __syncthreads();
+  const int count = (int)min((int64_t)kTile, (int64_t)n - tile0);
+#pragma unroll
+  for (int k = 0; k < kTileSteps; ++k) {
+    const int i = k * kSortThreads + t;
+    if (i >= count) break;
+    const int32_t ky = s_key[i], to = i + s_to[(ky >> shift) & (nd - 1)];
+    keys[to] = ky;
+    perm[to] = s_pos[i];
   }
 }
 
@@ -307,7 +373,7 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
       for (int i = es; i < ee; i += U) {
         rk::Pack<T, VEC> v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) v[j].load(g + (int64_t)s_pos[min(i + j, ee - 1)] * a.D + col);
+        for (int j = 0; j < U; ++j) v[j].load_once(g + (int64_t)s_pos[min(i + j, ee - 1)] * a.D + col);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
           if (i + j >= ee) break;
@@ -383,32 +449,78 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
   }
 }
 
+// acc += the head pieces of workgroups k0 .. k1, in that order, eight of them in flight
+template <int VEC>
+__device__ __forceinline__ void add_pieces(const SumArgs &a, int32_t k0, int32_t k1, int col, float (&acc)[VEC]) {
+  for (int32_t k = k0; k < k1; k += 8) {
+    rk::Pack<float, VEC> v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j].load(a.pieces + (int64_t)min(k + j, k1 - 1) * 2 * a.D + col);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (k + j >= k1) break;
+      float x[VEC];
+      v[j].widen(x);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += x[e];
+    }
+  }
+}
+
 // Rows that cross workgroups: the workgroup in which such a row begins has a tail piece, the ones it
 // goes on into have head pieces; they are added in that order.  One lane group per workgroup of the
 // summing launch; rows with many pieces are added by the whole workgroup, a consecutive share each.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict__ dW) {
   __shared__ float s_part[256 * VEC];
-  __shared__ int32_t s_last[256];                        // last workgroup of the row that begins in this one (0: none)
+  __shared__ int32_t s_last[kJoins];                       // last workgroup of the row that begins in this one (0: none)
+  __shared__ int32_t s_end;
   const int per_block = a.G * a.per_group;
   const int grp = threadIdx.x / a.L, l = threadIdx.x - grp * a.L;
-  const int32_t b = (int32_t)blockIdx.x * a.G + grp;
+  const int borders = min(a.G, kJoins);
+  const int32_t b = (int32_t)blockIdx.x * borders + grp;
   int32_t last = 0;
-  if (grp < a.G && (int64_t)(b + 1) * per_block < a.n) {
+  if (grp < borders && (int64_t)(b + 1) * per_block < a.n) {
     const int32_t s0 = b * per_block, s1 = s0 + per_block, key = a.keys[s1 - 1];
     const bool goes_on = key < a.rows && a.keys[s1] == key;
     const bool began_before = s0 > 0 && a.keys[s0 - 1] == key;
     if (goes_on && !began_before) {
-      const int32_t end = s1 + lower_bound(a.keys + s1, min(a.n - s1, per_block + 1), key + 1);
+      // how many of the next workgroups begin with the key, eight looked at together
       last = b + 1;
-      if (end - s1 > per_block) {                        // beyond the next workgroup: look for its end
-        const int32_t far = s1 + lower_bound(a.keys + s1, a.n - s1, key + 1);
-        last = (far - 1) / per_block;
+      bool open = true;
+      while (open && last - b < kLongRun) {
+        int32_t k[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) k[j] = a.keys[(int64_t)min(last + 1 + j, a.blocks - 1) * per_block];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          open = open && last + 1 < a.blocks && k[j] == key;
+          last += open ? 1 : 0;
+        }
       }
+      if (open) last = -1;                               // more than a lane group adds
     }
   }
-  if (grp < a.G && l == 0) s_last[grp] = last;
+  if (grp < borders && l == 0) s_last[grp] = last;
   __syncthreads();
+  for (int j = 0; j < borders; ++j) {                    // (the same for every thread: barriers inside)
+    if (s_last[j] >= 0) continue;
+    // the first workgroup that does not begin with the key, 256 looked at together
+    const int32_t bj = (int32_t)blockIdx.x * borders + j, key = a.keys[(int64_t)(bj + 1) * per_block - 1];
+    if (threadIdx.x == 0) s_end = INT32_MAX;
+    __syncthreads();
+    for (int32_t k0 = bj + 2;; k0 += 256) {
+      const int32_t k = k0 + (int32_t)threadIdx.x;
+      if (k >= a.blocks || a.keys[(int64_t)k * per_block] != key) atomicMin(&s_end, k);
+      __syncthreads();
+      const bool found = s_end != INT32_MAX;
+      __syncthreads();                                   // (nobody looks again before everybody has seen it)
+      if (found) break;
+    }
+    if (threadIdx.x == 0) s_last[j] = s_end - 1;
+    __syncthreads();
+  }
+  if (grp < borders) last = s_last[grp];
   for (int c0 = 0; c0 < a.D; c0 += a.L * VEC) {
     const bool on = grp < a.G && c0 + l * VEC < a.D;
     const int col = min(c0 + l * VEC, a.D - VEC);
@@ -417,27 +529,19 @@ __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict_
       const float *p = a.pieces + ((int64_t)b * 2 + 1) * a.D + col;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[e] = p[e];
-      for (int32_t k = b + 1; k <= last; ++k) {
-        const float *q = a.pieces + (int64_t)k * 2 * a.D + col;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += q[e];
-      }
+      add_pieces<VEC>(a, b + 1, last + 1, col, acc);
       put_row<T, VEC>(dW + (int64_t)a.keys[(int64_t)(b + 1) * per_block - 1] * a.D + col, acc, a.scale);
     }
-    for (int j = 0; j < a.G; ++j) {                      // (the same for every thread: barriers inside)
-      const int32_t bj = (int32_t)blockIdx.x * a.G + j, lj = s_last[j], pieces = lj - bj;
+    for (int j = 0; j < borders; ++j) {                  // (the same for every thread: barriers inside)
+      const int32_t bj = (int32_t)blockIdx.x * borders + j, lj = s_last[j], pieces = lj - bj;
       if (lj == 0 || pieces <= kLongRun) continue;
       const int32_t share = (pieces + a.G - 1) / a.G;
       if (on) {
         float acc[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-        const int32_t k0 = bj + 1 + grp * share, k1 = min(lj + 1, k0 + share);
-        for (int32_t k = k0; k < k1; ++k) {
-          const float *q = a.pieces + (int64_t)k * 2 * a.D + col;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[e] += q[e];
-        }
+        const int32_t k0 = bj + 1 + grp * share;
+        add_pieces<VEC>(a, k0, min(lj + 1, k0 + share), col, acc);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s_part[threadIdx.x * VEC + e] = acc[e];
       }
@@ -461,13 +565,14 @@ __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict_
 struct Layout {              // of the backward workspace, in 4-byte words
   int32_t L, G, per_group, blocks;
   int passes, bits;          // radix passes (0: the ids are sorted by counting) and bits of a digit
-  int32_t tile, tiles;
-  int64_t keys[2], perm[2], counts, pieces, words;
+  int32_t tiles;
+  int64_t keys[2], perm[2], counts, totals, pieces, words;
 };
 
 int lanes_of(int32_t D, int32_t dtype) {
   const int full = dtype == RK_F32 ? 4 : 8, vec = D >= full ? full : 1;
-  return std::min(256, (D + vec - 1) / vec);
+  // (four lanes at least: more than 64 rows side by side in a workgroup make long chains of joins)
+  return std::max(4, std::min(256, (D + vec - 1) / vec));
 }
 
 Layout layout_of(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
@@ -475,7 +580,7 @@ Layout layout_of(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
   y.L = lanes_of(D, dtype);
   y.G = 256 / y.L;
   // 512 entries for a workgroup where there are enough of them to give every CU some, fewer otherwise
-  y.per_group = std::max(4, std::min(32, 512 / y.G));
+  y.per_group = std::max(4, std::min(kPerGroup, 512 / y.G));
   while (y.per_group > 4 && rk::ceil_div(n, (int64_t)y.G * y.per_group) < 512) y.per_group /= 2;
   y.blocks = (int32_t)rk::ceil_div(n, (int64_t)y.G * y.per_group);
   if (n > kRankSortMax) {
@@ -483,8 +588,7 @@ Layout layout_of(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
     while ((rows >> key_bits) != 0) ++key_bits;          // keys are 0 .. rows
     y.passes = (int)rk::ceil_div(key_bits, kMaxDigitBits);
     y.bits = (int)rk::ceil_div(key_bits, y.passes);
-    y.tile = (int32_t)std::max<int64_t>(kMinTile, rk::ceil_div(rk::ceil_div(n, kMaxTiles), kSortThreads) * kSortThreads);
-    y.tiles = (int32_t)rk::ceil_div(n, y.tile);
+    y.tiles = (int32_t)rk::ceil_div(n, kTile);
   }
   int64_t at = 0;
   const int64_t room = rk::ceil_div(n, 4) * 4;
@@ -496,6 +600,8 @@ Layout layout_of(int64_t n, int32_t rows, int32_t D, int32_t dtype) {
   }
   y.counts = at;
   at += (int64_t)y.tiles << y.bits;
+  y.totals = at;
+  at += 1 << kMaxDigitBits;
   y.pieces = at;
   at += (int64_t)y.blocks * 2 * D;
   y.words = at;
@@ -510,27 +616,38 @@ int check_common(int32_t dtype, int32_t id_bytes, int64_t n, int32_t rows, int32
   return RK_OK;
 }
 
+template <typename T, int VEC, typename ID, int ROWS, bool ONCE>
+int launch_fwd_as(const void *W, int64_t ldw, int32_t rows, int32_t D, const void *ids, int64_t n, float scale, void *out,
+                  int L, hipStream_t st) {
+  const int64_t blocks = rk::ceil_div(n, (int64_t)(256 / L) * ROWS);
+  RK_CHECK_ARG(blocks < INT32_MAX, "too many ids");
+  emb_fwd_kernel<T, VEC, ID, ROWS, ONCE><<<(uint32_t)blocks, 256, 0, st>>>((const T *)W, ldw, rows, D, (const ID *)ids, n,
+                                                                         scale, L, (T *)out);
+  RK_CHECK_LAUNCH("emb_fwd_kernel");
+  return RK_OK;
+}
+
 template <typename T, int VEC, typename ID>
 int launch_fwd(const void *W, int64_t ldw, int32_t rows, int32_t D, const void *ids, int64_t n, float scale, void *out,
                int32_t dtype, hipStream_t st) {
-  const int L = lanes_of(D, dtype), G = 256 / L;
-  // four rows per lane group once that still fills the GPU: their loads are in flight together
-  const int per_thread = n >= (int64_t)G * 4 * 1024 ? 4 : 1;
-  const int64_t blocks = rk::ceil_div(n, (int64_t)G * per_thread);
-  RK_CHECK_ARG(blocks < INT32_MAX, "too many ids");
-  emb_fwd_kernel<T, VEC, ID><<<(uint32_t)blocks, 256, 0, st>>>((const T *)W, ldw, rows, D, (const ID *)ids, n, scale, L,
-                                                               per_thread, (T *)out);
-  RK_CHECK_LAUNCH("emb_fwd_kernel");
-  return RK_OK;
+  const int L = lanes_of(D, dtype);
+  // two rows per lane group once that still fills the GPU (2^20 rows of 256 bytes: 69 us; one 72, four 72, eight 73)
+  if (n < (int64_t)(256 / L) * 2 * 1024)
+    return launch_fwd_as<T, VEC, ID, 1, false>(W, ldw, rows, D, ids, n, scale, out, L, st);
+  if (n * D * (int64_t)sizeof(T) < kStreamBytes)
+    return launch_fwd_as<T, VEC, ID, 2, false>(W, ldw, rows, D, ids, n, scale, out, L, st);
+  return launch_fwd_as<T, VEC, ID, 2, true>(W, ldw, rows, D, ids, n, scale, out, L, st);
 }
 
 template <typename SRC>
 int launch_pass(SRC src, const Layout &y, int32_t n, int pass, int32_t *ws, int to, hipStream_t st) {
   const int shift = pass * y.bits;
-  emb_count_kernel<SRC><<<y.tiles, kSortThreads, 0, st>>>(src, n, y.tile, shift, y.bits, ws + y.counts);
+  emb_count_kernel<SRC><<<y.tiles, kSortThreads, 0, st>>>(src, n, shift, y.bits, ws + y.counts);
   RK_CHECK_LAUNCH("emb_count_kernel");
-  emb_place_kernel<SRC><<<y.tiles, kSortThreads, (size_t)kSortWaves * sizeof(int32_t) << y.bits, st>>>(
-      src, n, y.tile, shift, y.bits, ws + y.counts, ws + y.keys[to], ws + y.perm[to]);
+  emb_scan_kernel<<<(uint32_t)rk::ceil_div(1 << y.bits, 16), 256, 0, st>>>(ws + y.counts, y.tiles, 1 << y.bits, ws + y.totals);
+  RK_CHECK_LAUNCH("emb_scan_kernel");
+  emb_place_kernel<SRC><<<y.tiles, kSortThreads, 0, st>>>(src, n, shift, y.bits, ws + y.counts, ws + y.totals,
+                                                         ws + y.keys[to], ws + y.perm[to]);
   RK_CHECK_LAUNCH("emb_place_kernel");
   return RK_OK;
 }
@@ -539,7 +656,7 @@ int launch_pass(SRC src, const Layout &y, int32_t n, int pass, int32_t *ws, int 
 template <typename ID>
 int launch_sort(const ID *ids, int32_t n, int32_t rows, int64_t padding, const Layout &y, int32_t *ws, hipStream_t st) {
   if (y.passes == 0) {
-    emb_rank_sort_kernel<ID><<<(uint32_t)rk::ceil_div(n, 32), 256, 0, st>>>(ids, n, rows, padding, ws + y.keys[0],
+    emb_rank_sort_kernel<ID><<<(uint32_t)rk::ceil_div(n, 256 / kRankThreads), 256, 0, st>>>(ids, n, rows, padding, ws + y.keys[0],
                                                                            ws + y.perm[0]);
     RK_CHECK_LAUNCH("emb_rank_sort_kernel");
     return RK_OK;
@@ -559,7 +676,7 @@ int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
   emb_sum_kernel<T, VEC><<<(uint32_t)blocks, 256, 0, st>>>(a, (const T *)g, (T *)dW);
   RK_CHECK_LAUNCH("emb_sum_kernel");
   if (a.blocks > 1) {
-    emb_join_kernel<T, VEC><<<(uint32_t)rk::ceil_div(a.blocks - 1, a.G), 256, 0, st>>>(a, (T *)dW);
+    emb_join_kernel<T, VEC><<<(uint32_t)rk::ceil_div(a.blocks - 1, std::min(a.G, kJoins)), 256, 0, st>>>(a, (T *)dW);
     RK_CHECK_LAUNCH("emb_join_kernel");
   }
   return RK_OK;

@@ -175,8 +175,9 @@ def preference_loss(scores, items, ref_logps, beta=0.1, label_smoothing=0.0, kin
         raise ValueError(f"preference_loss: one reference log-probability per list, got {tuple(ref_logps.shape)} for {S}")
     items = ops._list_args(scores, items, "preference_loss")
     ops._same_device(scores, ref_logps)
-    logps, loss = ops._ListLogps.apply(scores, items, ops._f32c(ref_logps.detach()), int(ignore_index), int(bool(average)),
-                                       float(beta), float(label_smoothing), _PREFERENCE_KINDS[kind])
+    logps, loss = ops._ListLogps.apply(scores, items, ops._f32c(ref_logps.detach()),
+                                       (int(ignore_index), int(bool(average)), float(beta), float(label_smoothing),
+                                        _PREFERENCE_KINDS[kind]))
     return loss, logps
 
 

@@ -423,42 +423,54 @@ def _scratch(nbytes, device):
 
 
 def _same_device(*tensors):
-    """All of them on one HIP device (None is skipped)."""
+    """All of them on one HIP device."""
     _need_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
+    dev = tensors[0].device
+    for t in tensors[1:]:
+        if t.device != dev:
+            raise ValueError(f"tensors on several devices: {dev} and {t.device}")
+
+
+def _once(backward):
+    """A backward pass without a derivative of its own, as torch's once_differentiable, whose bookkeeping is
+    entered only where a graph of the gradient is asked for."""
+    slow = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 class _EmbeddingLookup(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, ids, scale, padding_idx):
-        out = _embedding_fwd(weight, ids, scale)
+    def forward(ctx, weight, ids, args):       # args: (scale, padding_idx)
         ctx.save_for_backward(ids)
-        ctx.args = (weight.shape, scale, padding_idx)
-        return out
+        ctx.args, ctx.shape = args, weight.shape
+        return _embedding_fwd(weight, ids, args[0])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g):
         ids, = ctx.saved_tensors
-        (rows, D), scale, padding_idx = ctx.args
+        (rows, D), (scale, padding_idx) = ctx.shape, ctx.args
         g = g.contiguous()
-        dw = torch.empty((rows, D), dtype=g.dtype, device=g.device)
-        kind = _ELEM[g.dtype]
-        n = ids.numel()
-        ws = _scratch(_ffi.load().rk_embedding_bwd_ws_bytes(n, rows, D, kind), g.device)
-        _ffi.call_on(g.device, "rk_embedding_bwd", ptr(g), kind, ptr(ids), ids.element_size(), n, rows, D, scale,
-                     padding_idx, ptr(dw), ptr(ws), ws.numel() * 8, stream_ptr(g.device))
-        return dw, None, None, None
+        dev, kind, n = g.device, _ELEM[g.dtype], ids.numel()
+        dw = torch.empty((rows, D), dtype=g.dtype, device=dev)
+        ws = _scratch(_ffi.load().rk_embedding_bwd_ws_bytes(n, rows, D, kind), dev)
+        _ffi.call_on(dev, "rk_embedding_bwd", g.data_ptr(), kind, ids.data_ptr(), ids.element_size(), n, rows, D, scale,
+                     padding_idx, dw.data_ptr(), ws.data_ptr(), ws.numel() * 8)
+        return dw, None, None
 
 
-def _embedding_fwd(weight, ids, scale):
-    rows, D = weight.shape
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= D else weight.contiguous()
-    out = torch.empty((*ids.shape, D), dtype=w.dtype, device=w.device)
-    _ffi.call_on(w.device, "rk_embedding_fwd", ptr(w), w.stride(0), rows, D, _ELEM[w.dtype], ptr(ids),
-                 ids.element_size(), ids.numel(), scale, ptr(out), stream_ptr(w.device))
+def _embedding_fwd(w, ids, scale):
+    rows, D = w.shape
+    ld, step = w.stride()
+    if step != 1 or ld < D:
+        w, ld = w.contiguous(), D
+    dev = w.device
+    out = torch.empty((*ids.shape, D), dtype=w.dtype, device=dev)
+    _ffi.call_on(dev, "rk_embedding_fwd", w.data_ptr(), ld, rows, D, _ELEM[w.dtype], ids.data_ptr(), ids.element_size(),
+                 ids.numel(), scale, out.data_ptr())
     return out
 
 
@@ -472,20 +484,21 @@ def embedding_lookup(weight, ids, scale=1.0, padding_idx=None):
     torch.nn.Embedding) add nothing.  An id outside the table gives a row of NaN and no gradient."""
     if weight.dim() != 2 or weight.shape[1] < 1:
         raise ValueError(f"embedding_lookup: the table is [rows, D], got {tuple(weight.shape)}")
-    _elem(weight, "embedding_lookup")
-    if ids.dtype not in (torch.int32, torch.int64):
+    if weight.dtype not in _ELEM:
+        _elem(weight, "embedding_lookup")
+    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
         raise ValueError(f"embedding_lookup: ids are int32 or int64, not {ids.dtype}")
-    rows = weight.shape[0]
     if padding_idx is None:
         padding_idx = -1
     else:
+        rows = weight.shape[0]
         if not -rows <= padding_idx < rows:
             raise ValueError(f"embedding_lookup: padding_idx {padding_idx} outside the table of {rows} rows")
         padding_idx = int(padding_idx) % rows
     _same_device(weight, ids)
     ids = ids.contiguous()
     if weight.requires_grad and torch.is_grad_enabled():
-        return _EmbeddingLookup.apply(weight, ids, float(scale), padding_idx)
+        return _EmbeddingLookup.apply(weight, ids, (float(scale), padding_idx))
     return _embedding_fwd(weight.detach(), ids, float(scale))
 
 
@@ -494,10 +507,11 @@ PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = 0, 1, 2   # RK_PREF_* of the header
 
 def _list_args(scores, items, what):
     """Checks a list operator's scores and items; returns the items as contiguous int64."""
-    _elem(scores, what)
-    if items.dtype not in (torch.int32, torch.int64):
+    if scores.dtype not in _ELEM:
+        _elem(scores, what)
+    if items.dtype != torch.int64 and items.dtype != torch.int32:
         raise ValueError(f"{what}: items are int32 or int64, not {items.dtype}")
-    if scores.dim() not in (2, 3) or tuple(scores.shape[:-1]) != tuple(items.shape):
+    if scores.dim() not in (2, 3) or scores.shape[:-1] != items.shape:
         raise ValueError(f"{what}: scores [lists, places, catalogue] and items [lists, places] (or without places), "
                          f"got {tuple(scores.shape)} and {tuple(items.shape)}")
     if 0 in scores.shape[1:]:
@@ -508,61 +522,68 @@ def _list_args(scores, items, what):
 
 def _list_geometry(scores, items):
     """Arguments that describe scores and items to the rk_list_logps_* / rk_preference_* calls."""
-    S, V = scores.shape[0], scores.shape[-1]
-    T = scores.shape[1] if scores.dim() == 3 else 1
-    return (ptr(scores), _ELEM[scores.dtype], S, T, V, scores.stride(0), scores.stride(1) if scores.dim() == 3 else 0,
-            ptr(items), T)
-
-
-def _rows_contiguous(scores):
-    return scores if scores.stride(-1) == 1 or scores.shape[-1] == 1 else scores.contiguous()
+    if scores.dim() == 3:
+        (S, T, V), (ss, st, _) = scores.shape, scores.stride()
+    else:
+        (S, V), (ss, _), T, st = scores.shape, scores.stride(), 1, 0
+    return scores.data_ptr(), _ELEM[scores.dtype], S, T, V, ss, st, items.data_ptr(), T
 
 
 class _ListLogps(torch.autograd.Function):
     """logps [S]; with ref_logps also the preference loss of the pairs (s, S/2 + s)."""
 
     @staticmethod
-    def forward(ctx, scores, items, ref, ignore_index, average, beta, smoothing, kind):
-        scores = _rows_contiguous(scores)
-        dev, S, rows = scores.device, scores.shape[0], items.numel()
-        # (max, log sum) of every row, used places and slopes of every list: kept for the backward pass
-        keep = torch.empty(2 * rows + 2 * S, dtype=torch.float32, device=dev)
-        base = keep.data_ptr()
-        stat, used, slope = base, base + 8 * rows, base + 8 * rows + 4 * S
-        logps = torch.empty(S, dtype=torch.float32, device=dev)
-        loss = None
-        if S:
-            geo = _list_geometry(scores, items)
-            ws = _scratch(_ffi.load().rk_list_logps_ws_bytes(*geo[2:5]), dev)
-            tail = (ptr(ws), ws.numel() * 8, stream_ptr(dev))
-            if ref is None:
-                _ffi.call_on(dev, "rk_list_logps_fwd", *geo, ignore_index, average, stat, ptr(logps), used, *tail)
-            else:
-                loss = torch.empty((), dtype=torch.float32, device=dev)
-                _ffi.call_on(dev, "rk_preference_fwd", *geo, ignore_index, average, ptr(ref), beta, smoothing, kind, stat,
-                             ptr(logps), used, slope, ptr(loss), *tail)
-        ctx.save_for_backward(scores, items, keep)
-        ctx.args = (ignore_index, average, ref is not None)
+    def forward(ctx, scores, items, ref, args):      # args: (ignore_index, average, beta, label_smoothing, kind)
+        if scores.stride(-1) != 1 and scores.shape[-1] != 1:
+            scores = scores.contiguous()
+        geo = _list_geometry(scores, items)
+        dev, S, rows = scores.device, geo[2], items.numel()
         ctx.set_materialize_grads(False)
-        return (logps,) if ref is None else (logps, loss)
+        ignore_index, average, beta, smoothing, kind = args
+        ctx.args = (ignore_index, average, ref is not None)
+        logps = torch.empty(S, dtype=torch.float32, device=dev)
+        if S == 0:
+            ctx.save_for_backward(scores, items, logps)
+            return (logps,)
+        # (max, log sum) of every row, used places and slopes of every list: kept for the backward pass;
+        # behind them the call's workspace
+        n_keep = 2 * rows + 2 * S
+        n_keep += n_keep % 2
+        ws_bytes = _ffi.load().rk_list_logps_ws_bytes(S, geo[3], geo[4])
+        keep = torch.empty(n_keep + (ws_bytes + 3) // 4, dtype=torch.float32, device=dev)
+        ctx.save_for_backward(scores, items, keep)
+        stat = keep.data_ptr()
+        used, ws = stat + 8 * rows, stat + 4 * n_keep
+        if ref is None:
+            _ffi.call_on(dev, "rk_list_logps_fwd", *geo, ignore_index, average, stat, logps.data_ptr(), used, ws, ws_bytes)
+            return (logps,)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        _ffi.call_on(dev, "rk_preference_fwd", *geo, ignore_index, average, ref.data_ptr(), beta, smoothing, kind, stat,
+                     logps.data_ptr(), used, used + 4 * S, loss.data_ptr(), ws, ws_bytes)
+        return logps, loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g_logps, g_loss=None):
         scores, items, keep = ctx.saved_tensors
         ignore_index, average, pairs = ctx.args
         if g_logps is None and g_loss is None:
-            return (None,) * 8
-        dev, S, rows = scores.device, scores.shape[0], items.numel()
-        g_logps = _f32c(g_logps) if g_logps is not None else None
-        g_loss = _f32c(g_loss) if g_loss is not None else None
+            return (None,) * 4
+        dev = scores.device
         dx = torch.empty(scores.shape, dtype=scores.dtype, device=dev)
+        geo = _list_geometry(scores, items)
+        S = geo[2]
         if S:
-            base = keep.data_ptr()
-            _ffi.call_on(dev, "rk_list_logps_bwd", *_list_geometry(scores, items), ignore_index, average, base,
-                         base + 8 * rows, ptr(g_loss), base + 8 * rows + 4 * S if pairs else None, ptr(g_logps), ptr(dx),
-                         stream_ptr(dev))
-        return (dx,) + (None,) * 7
+            if g_logps is not None:
+                g_logps = _f32c(g_logps)
+            if g_loss is not None:
+                g_loss = _f32c(g_loss)
+            stat = keep.data_ptr()
+            used = stat + 8 * items.numel()
+            _ffi.call_on(dev, "rk_list_logps_bwd", *geo, ignore_index, average, stat, used,
+                         None if g_loss is None else g_loss.data_ptr(), used + 4 * S if pairs else None,
+                         None if g_logps is None else g_logps.data_ptr(), dx.data_ptr())
+        return dx, None, None, None
 
 
 def list_logps(scores, items, ignore_index=-100, average=False):
@@ -574,7 +595,7 @@ def list_logps(scores, items, ignore_index=-100, average=False):
     not read and get a gradient of zero).  A list without places in use has 0; an item outside the
     catalogue makes its list NaN.  Returns fp32 [S], differentiable with respect to scores."""
     items = _list_args(scores, items, "list_logps")
-    return _ListLogps.apply(scores, items, None, int(ignore_index), int(bool(average)), 0.0, 0.0, 0)[0]
+    return _ListLogps.apply(scores, items, None, (int(ignore_index), int(bool(average)), 0.0, 0.0, 0))[0]
 
 
 # --------------------------------------------------------------------------
