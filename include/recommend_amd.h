@@ -378,8 +378,9 @@ int rk_list_logps_bwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
                       void *stream);
 
 /* ---- AdamW over many tensors, moments in 32 or 8 bits ---------------------- */
-/* The reference's AdamW choice (train/graph_trainer.py:78-101) with clip_grad_norm_ (:151-156), in two
- * launches per 48 tensors; nothing is allocated, so a call can be recorded in a HIP graph.
+/* The reference's AdamW choice (train/graph_trainer.py:78-101) with clip_grad_norm_ (:151-156): one
+ * small launch, and one (with clipping: two) per 48 tensors; nothing is allocated, so a call can be
+ * recorded in a HIP graph.
  *   g = min(1, max_norm / (|grads| + 1e-6)) * grad           (max_norm <= 0: no clipping)
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p - lr wd p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
@@ -390,8 +391,7 @@ int rk_list_logps_bwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
  * sqrt(v) that is not zero is at least the smallest code.
  * lr: device array of n_groups floats; step: device counter, incremented by the call; norm_out (may
  * be NULL): the gradients' 2-norm before clipping, written when max_norm > 0.  ws:
- * rk_adamw_ws_bytes() bytes, 16-byte aligned, zeroed once by the caller and left ready for the next
- * call; calls that share it must not overlap in time. */
+ * rk_adamw_ws_bytes() bytes of scratch, 16-byte aligned. */
 #define RK_ADAMW_BLOCK 64
 #define RK_ADAMW_MAX_GROUPS 8
 typedef struct rk_adamw_tensor {

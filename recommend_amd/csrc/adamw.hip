@@ -1,13 +1,15 @@
-// AdamW over a list of tensors in two launches, with 32-bit or 8-bit moments, parameters and gradients
+// AdamW over a list of tensors in two or three launches, with 32-bit or 8-bit moments, parameters and gradients
 // in fp32, bfloat16 or fp16, several parameter groups and global-norm clipping (gfx950).
 //
 //   g = coef * grad                      coef = min(1, max_norm / (|grad| + 1e-6)) over all tensors
 //   m = beta1 m + (1 - beta1) g          v = beta2 v + (1 - beta2) g^2
 //   p = p - lr wd p - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 //
-// Launch 1 advances the step count, adds up the squared gradients (in 64 bits, when clipping is asked
-// for; the workgroup that finishes last joins the partial sums in order) and leaves the step's factors
-// in the workspace.  Launch 2 updates.  The descriptors travel by value in the kernels' arguments
+// Where clipping is asked for, the first launch adds up the squared gradients, in 64 bits, one partial
+// sum per workgroup.  The next one, a single workgroup, advances the step count, joins the partial sums
+// in order and leaves the step's factors in the workspace.  The last one updates.  (Joining in the
+// workgroup that finishes the norm last saves the small launch, but its release fences write back the
+// L2 once per workgroup: 158 us instead of 60 for 185 MB.)  The descriptors travel by value in the kernels' arguments
 // (kMaxTensors per launch): nothing is copied or allocated, so a step can be recorded in a HIP graph.
 //
 // 8-bit moments: blocks of 64 consecutive elements share an fp32 scale; m and the root of v are held as
@@ -27,8 +29,9 @@ namespace {
 
 constexpr int kMaxTensors = 48;
 constexpr int kMaxGroups = RK_ADAMW_MAX_GROUPS;
-constexpr int kChunk = 4096;         // elements of a workgroup of the update
-constexpr int kNormBlocks = 1024;    // workgroups of the squared-norm launch
+constexpr int kChunk = 2048;         // elements of a workgroup of the update
+constexpr int kNormChunk = 8192;     // elements that a workgroup of the squared-norm launch takes at a time
+constexpr int kNormBlocks = 2048;    // its workgroups
 constexpr int kBlock = RK_ADAMW_BLOCK;
 constexpr float kFull = 448.0f;      // largest finite e4m3 value
 constexpr float kTiny = 1e-30f;      // block maxima below this count as this
@@ -68,12 +71,20 @@ struct Factors {                      // what launch 1 leaves for launch 2
   float step_size[kMaxGroups], inv_root_bc2[kMaxGroups], decay[kMaxGroups];
 };
 
+// x^t by squaring: a dozen instructions where pow() costs the kernel a third of its registers
+__device__ __forceinline__ double power(double x, int64_t t) {
+  double y = 1.0;
+  for (; t > 0; t >>= 1, x *= x)
+    if (t & 1) y *= x;
+  return y;
+}
+
 __device__ __forceinline__ void write_factors(const GroupsIn &gr, const float *__restrict__ lr, int64_t t, double norm,
                                               float max_norm, float *__restrict__ norm_out, Factors *__restrict__ f) {
   // 1 - beta^t in 64 bits: in 32 it has lost four digits in the first steps
   for (int g = threadIdx.x; g < gr.n; g += (int)blockDim.x) {
-    f->step_size[g] = (float)((double)lr[g] / (1.0 - pow(gr.g[g].beta1, (double)t)));
-    f->inv_root_bc2[g] = (float)(1.0 / sqrt(1.0 - pow(gr.g[g].beta2, (double)t)));
+    f->step_size[g] = (float)((double)lr[g] / (1.0 - power(gr.g[g].beta1, t)));
+    f->inv_root_bc2[g] = (float)(1.0 / sqrt(1.0 - power(gr.g[g].beta2, t)));
     f->decay[g] = (float)((double)lr[g] * gr.g[g].weight_decay);
   }
   if (threadIdx.x == 0) {
@@ -83,56 +94,70 @@ __device__ __forceinline__ void write_factors(const GroupsIn &gr, const float *_
   }
 }
 
-__global__ __launch_bounds__(64) void adamw_begin_kernel(GroupsIn gr, const float *__restrict__ lr,
-                                                         int64_t *__restrict__ step, Factors *__restrict__ f) {
+// One workgroup: the step count, the gradients' norm from the partial sums of the norm launches (in
+// order), the step's factors.
+__global__ __launch_bounds__(256) void adamw_begin_kernel(GroupsIn gr, const float *__restrict__ lr,
+                                                          int64_t *__restrict__ step, const double *__restrict__ partial,
+                                                          int32_t n_partial, float max_norm, float *__restrict__ norm_out,
+                                                          Factors *__restrict__ f) {
+  __shared__ double red[4];
   const int64_t t = step[0] + 1;
+  double s = 0.0;
+#pragma unroll 8
+  for (int32_t i = threadIdx.x; i < n_partial; i += 256) s += partial[i];
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, rk::kWave);
+  if (threadIdx.x % rk::kWave == 0) red[threadIdx.x / rk::kWave] = s;
   __syncthreads();
   if (threadIdx.x == 0) step[0] = t;
-  write_factors(gr, lr, t, 0.0, 0.0f, nullptr, f);
+  write_factors(gr, lr, t, sqrt((red[0] + red[1]) + (red[2] + red[3])), max_norm, norm_out, f);
 }
 
+// sum of squares of g[lo .. hi) (a chunk), in 64 bits, all vectors of a lane in flight
 template <typename T>
 __device__ __forceinline__ double square_sum(const T *__restrict__ g, int64_t lo, int64_t hi) {
-  constexpr int VEC = rk::Elem<T>::kVec;
-  double s = 0.0;
+  constexpr int VEC = rk::Elem<T>::kVec, U = kNormChunk / (256 * VEC);
+  double s[2] = {0.0, 0.0};
   int64_t i = lo + (int64_t)threadIdx.x * VEC;
-  for (; i + VEC <= hi; i += 256 * VEC) {
-    rk::Pack<T, VEC> v;
-    v.load(g + i);
-    float f[VEC];
-    v.widen(f);
+  for (; i + (U - 1) * 256 * VEC + VEC <= hi; i += U * 256 * VEC) {
+    rk::Pack<T, VEC> v[U];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) s = fma((double)f[e], (double)f[e], s);
+    for (int u = 0; u < U; ++u) v[u].load(g + i + u * 256 * VEC);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      v[u].widen(f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s[e & 1] = fma((double)f[e], (double)f[e], s[e & 1]);
+    }
   }
-  for (int e = 0; e < VEC && i + e < hi; ++e) {
-    const double x = (double)rk::Elem<T>::get(g[i + e]);
-    s = fma(x, x, s);
+  for (; i < hi; i += 256 * VEC) {
+    float f[VEC];
+    if (i + VEC <= hi) {
+      rk::Pack<T, VEC> v;
+      v.load(g + i);
+      v.widen(f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = i + e < hi ? rk::Elem<T>::get(g[i + e]) : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) s[e & 1] = fma((double)f[e], (double)f[e], s[e & 1]);
   }
-  return s;
+  return s[0] + s[1];
 }
 
-__device__ __forceinline__ int find_tensor(const Args &a, int32_t chunk) {
-  int i = 0;
-  while (i + 1 < a.n && a.chunk_start[i + 1] <= chunk) ++i;
-  return i;
-}
-
-// Squared gradients of one launch's tensors, one partial sum per workgroup; the last workgroup of the
-// last launch (n_partial > 0) joins all of them in order and writes the factors.  The partial sums are
-// stored and read with agent scope around the ticket: the workgroups run under different L2 caches.
-__global__ __launch_bounds__(256) void adamw_norm_kernel(Args a, double *__restrict__ partial, int32_t first,
-                                                         int32_t n_partial, int32_t *__restrict__ ticket, GroupsIn gr,
-                                                         const float *__restrict__ lr, int64_t *__restrict__ step,
-                                                         float max_norm, float *__restrict__ norm_out,
-                                                         Factors *__restrict__ f) {
+// Squared gradients of one launch's tensors, one partial sum per workgroup.  Neighbouring workgroups read
+// neighbouring chunks: with a consecutive share for each they met on the same memory channels (433 MB in
+// 208 us instead of 110).
+__global__ __launch_bounds__(256) void adamw_norm_kernel(Args a, double *__restrict__ partial) {
   __shared__ double red[4];
-  __shared__ int s_last;
   double s = 0.0;
   const int32_t chunks = a.chunk_start[a.n];
-  for (int32_t c = blockIdx.x; c < chunks; c += (int32_t)gridDim.x) {
-    const int i = find_tensor(a, c);
+  for (int32_t c = blockIdx.x, i = 0; c < chunks; c += (int32_t)gridDim.x) {
+    while (a.chunk_start[i + 1] <= c) ++i;
     const Tensor &t = a.t[i];
-    const int64_t lo = (int64_t)(c - a.chunk_start[i]) * kChunk, hi = min(t.n, lo + kChunk);
+    const int64_t lo = (int64_t)(c - a.chunk_start[i]) * kNormChunk, hi = min(t.n, lo + kNormChunk);
     const int gd = t.kind >> 2;
     if (gd == RK_F32)
       s += square_sum((const float *)t.grad, lo, hi);
@@ -145,41 +170,33 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(Args a, double *__restr
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, rk::kWave);
   if (threadIdx.x % rk::kWave == 0) red[threadIdx.x / rk::kWave] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(&partial[first + blockIdx.x], (red[0] + red[1]) + (red[2] + red[3]), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
-    s_last = n_partial > 0 &&
-             __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  double all = 0.0;
-  for (int32_t i = threadIdx.x; i < n_partial; i += 256)
-    all += __hip_atomic_load(&partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, rk::kWave);
-  if (threadIdx.x % rk::kWave == 0) red[threadIdx.x / rk::kWave] = all;
-  const int64_t t = step[0] + 1;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    step[0] = t;
-    ticket[0] = 0;                    // ready for the next step
-  }
-  write_factors(gr, lr, t, sqrt((red[0] + red[1]) + (red[2] + red[3])), max_norm, norm_out, f);
+  if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// largest value of a row of 16 lanes, in all of them
-__device__ __forceinline__ float row_max16(float x) {
-#define RK_ROW_MAX(CTRL) \
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), CTRL, 0xF, 0xF, false)))
+// Largest of non-negative floats over a row of 16 lanes, in all of them.  As integers: the order of
+// non-negative floats is that of their bits, and a NaN is larger than all (so it reaches the block's
+// scale), without the extra instructions that quiet a float maximum's operands.
+__device__ __forceinline__ uint32_t row_max16(uint32_t x) {
+#define RK_ROW_MAX(CTRL) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, false))
   RK_ROW_MAX(0x128);   // row_ror:8
   RK_ROW_MAX(0x124);
   RK_ROW_MAX(0x122);
   RK_ROW_MAX(0x121);
 #undef RK_ROW_MAX
   return x;
+}
+
+// 1 / x and sqrt(x) rounded to nearest in a few instructions: the hardware's approximation and one
+// correction with the exact residual.  Equal to the correctly rounded results for every significand
+// (checked over all of them, at exponents from -100 to 100); unlike the compiler's expansions they do not
+// care for subnormal x, whose roots (below 2^-63) are zero to an update.
+__device__ __forceinline__ float exact_rcp(float x) {
+  const float y = __builtin_amdgcn_rcpf(x);
+  return fmaf(fmaf(-x, y, 1.0f), y, y);
+}
+__device__ __forceinline__ float exact_sqrt(float x) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-126f)), s = x * y;
+  return fmaf(fmaf(-s, s, x), 0.5f * y, s);
 }
 
 __device__ __forceinline__ uint32_t encode4(const float (&x)[4]) {
@@ -194,131 +211,159 @@ __device__ __forceinline__ void decode4(uint32_t w, float scale, float (&x)[4]) 
   x[3] = hi[1] * scale;
 }
 
-// Four consecutive elements per lane and step: 16 lanes hold one block of 64.
-template <typename PT, typename GT, bool Q8>
-__device__ __forceinline__ void update(const Tensor &t, int64_t lo, int64_t hi, const Hyper &h, const Factors &f, int group) {
+// Four consecutive elements per lane and step: 16 lanes hold one block of 64.  FULL: the whole chunk
+// lies in the tensor (i.e. all but a tensor's last).
+template <typename PT, typename GT, bool Q8, bool FULL>
+__device__ __forceinline__ void update(const Tensor &t, int64_t chunk, const Hyper &h, const Factors &f, int group) {
   constexpr int U = kChunk / 1024;
-  PT *__restrict__ P = (PT *)t.param;
-  const GT *__restrict__ G = (const GT *)t.grad;
-  float p[U][4], g[U][4], m[U][4], v[U][4];
+  const int left = FULL ? kChunk : (int)(t.n - chunk);     // elements of the tensor from the chunk on
+  PT *__restrict__ P = (PT *)t.param + chunk;
+  const GT *__restrict__ G = (const GT *)t.grad + chunk;
+  float *__restrict__ M = (float *)t.m + chunk, *__restrict__ V = (float *)t.v + chunk;
+  uint32_t *__restrict__ CM = (uint32_t *)t.m + chunk / 4, *__restrict__ CV = (uint32_t *)t.v + chunk / 4;
+  float *__restrict__ SM = t.m_scale + chunk / kBlock, *__restrict__ SV = t.v_scale + chunk / kBlock;
+  rk::Pack<PT, 4> p[U];
+  rk::Pack<GT, 4> g[U];
+  rk::Pack<float, 4> m[U], v[U];
+  uint32_t cm[U], cv[U];
+  float sm[U], sv[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t i = lo + u * 1024 + (int64_t)threadIdx.x * 4;
-    if (i + 4 <= hi) {
-      rk::Pack<PT, 4> a;
-      a.load(P + i);
-      a.widen(p[u]);
-      rk::Pack<GT, 4> b;
-      b.load(G + i);
-      b.widen(g[u]);
+    const int i = u * 1024 + (int)threadIdx.x * 4;
+    if (FULL || i + 4 <= left) {
+      p[u].load_once(P + i);
+      g[u].load_once(G + i);
       if constexpr (!Q8) {
-        rk::Pack<float, 4> c;
-        c.load((const float *)t.m + i);
-        c.widen(m[u]);
-        c.load((const float *)t.v + i);
-        c.widen(v[u]);
+        m[u].load_once(M + i);
+        v[u].load_once(V + i);
       }
     } else {
+      float x[4], y[4], z[4], w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool in = i + e < hi;
-        p[u][e] = in ? rk::Elem<PT>::get(P[i + e]) : 0.0f;
-        g[u][e] = in ? rk::Elem<GT>::get(G[i + e]) : 0.0f;
-        if constexpr (!Q8) {
-          m[u][e] = in ? ((const float *)t.m)[i + e] : 0.0f;
-          v[u][e] = in ? ((const float *)t.v)[i + e] : 0.0f;
-        }
+        const bool in = i + e < left;
+        x[e] = in ? rk::Elem<PT>::get(P[i + e]) : 0.0f;
+        y[e] = in ? rk::Elem<GT>::get(G[i + e]) : 0.0f;
+        z[e] = !Q8 && in ? M[i + e] : 0.0f;
+        w[e] = !Q8 && in ? V[i + e] : 0.0f;
       }
+      p[u].narrow(x);
+      g[u].narrow(y);
+      m[u].narrow(z);
+      v[u].narrow(w);
     }
     if constexpr (Q8) {
-      if (i < hi) {                   // (the codes are padded to whole blocks)
-        const int64_t b = i / kBlock;
-        decode4(((const uint32_t *)t.m)[i / 4], t.m_scale[b], m[u]);
-        decode4(((const uint32_t *)t.v)[i / 4], t.v_scale[b], v[u]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[u][e] *= v[u][e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m[u][e] = v[u][e] = 0.0f;
-      }
+      const bool in = FULL || i < left;                    // (the codes are padded to whole blocks)
+      cm[u] = in ? CM[i / 4] : 0u;
+      cv[u] = in ? CV[i / 4] : 0u;
+      sm[u] = in ? SM[i / kBlock] : 0.0f;
+      sv[u] = in ? SV[i / kBlock] : 0.0f;
     }
   }
   const float coef = f.coef, step_size = f.step_size[group], inv_root = f.inv_root_bc2[group], decay = f.decay[group];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t i = lo + u * 1024 + (int64_t)threadIdx.x * 4;
-    float r[4];
+    const int i = u * 1024 + (int)threadIdx.x * 4;
+    float x[4], d[4], a[4], b[4], r[4];
+    p[u].widen(x);
+    g[u].widen(d);
+    if constexpr (Q8) {
+      decode4(cm[u], sm[u], a);
+      decode4(cv[u], sv[u], b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] *= b[e];
+    } else {
+      m[u].widen(a);
+      v[u].widen(b);
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float x = g[u][e] * coef;
-      m[u][e] = m[u][e] * h.beta1 + x * h.one_minus_beta1;
-      v[u][e] = v[u][e] * h.beta2 + (x * x) * h.one_minus_beta2;
-      r[e] = sqrtf(v[u][e]);
-      // (the reciprocal is good to one unit in the last place, and the update is small beside p)
-      const float q = p[u][e] - p[u][e] * decay;
-      p[u][e] = q - step_size * (m[u][e] * __builtin_amdgcn_rcpf(r[e] * inv_root + h.eps));
+      const float y = d[e] * coef;
+      a[e] = a[e] * h.beta1 + y * h.one_minus_beta1;
+      b[e] = b[e] * h.beta2 + (y * y) * h.one_minus_beta2;
+      r[e] = Q8 ? exact_sqrt(b[e]) : sqrtf(b[e]);
+      // (fused where the result is only p: rounded once less, and the reciprocal is good to a unit in the last place)
+      const float q = fmaf(-x[e], decay, x[e]);
+      x[e] = fmaf(-step_size, a[e] * __builtin_amdgcn_rcpf(fmaf(r[e], inv_root, h.eps)), q);
     }
-    if (i + 4 <= hi) {
-      rk::Pack<PT, 4> a;
-      a.narrow(p[u]);
-      a.store(P + i);
+    if (FULL || i + 4 <= left) {
+      p[u].narrow(x);
+      p[u].store_once(P + i);
       if constexpr (!Q8) {
-        rk::Pack<float, 4> c;
-        c.narrow(m[u]);
-        c.store((float *)t.m + i);
-        c.narrow(v[u]);
-        c.store((float *)t.v + i);
+        m[u].narrow(a);
+        m[u].store_once(M + i);
+        v[u].narrow(b);
+        v[u].store_once(V + i);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (i + e >= hi) {
-          m[u][e] = r[e] = 0.0f;
+        if (i + e >= left) {
+          a[e] = r[e] = 0.0f;
           continue;
         }
-        P[i + e] = rk::Elem<PT>::put(p[u][e]);
+        P[i + e] = rk::Elem<PT>::put(x[e]);
         if constexpr (!Q8) {
-          ((float *)t.m)[i + e] = m[u][e];
-          ((float *)t.v)[i + e] = v[u][e];
+          M[i + e] = a[e];
+          V[i + e] = b[e];
         }
       }
     }
     if constexpr (Q8) {
       // (every lane of a row takes part in its maximum, those behind the end with zeros)
-      const float am = fmaxf(row_max16(fmaxf(fmaxf(fabsf(m[u][0]), fabsf(m[u][1])), fmaxf(fabsf(m[u][2]), fabsf(m[u][3])))), kTiny);
-      const float ar = fmaxf(row_max16(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]))), kTiny);
-      const float im = (1.0f / am) * kFull, ir = (1.0f / ar) * kFull;
-      float x[4], y[4];
+      uint32_t ua[4], ur[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[e] = m[u][e] * im;
-        y[e] = r[e] * ir;
-        if (r[e] > 0.0f) y[e] = fmaxf(y[e], 0.001953125f);   // 2^-9, the smallest code above zero
+        ua[e] = __float_as_uint(a[e]) & 0x7FFFFFFFu;
+        ur[e] = __float_as_uint(r[e]) & 0x7FFFFFFFu;
       }
-      if (i < hi) {
-        ((uint32_t *)t.m)[i / 4] = encode4(x);
-        ((uint32_t *)t.v)[i / 4] = encode4(y);
+      const uint32_t tiny = __float_as_uint(kTiny);
+      const float am = __uint_as_float(max(row_max16(max(max(ua[0], ua[1]), max(ua[2], ua[3]))), tiny));
+      const float ar = __uint_as_float(max(row_max16(max(max(ur[0], ur[1]), max(ur[2], ur[3]))), tiny));
+      const float im = exact_rcp(am) * kFull, ir = exact_rcp(ar) * kFull;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] *= im;
+        // a root above zero gets the smallest code, 2^-9, at least: the median of a huge number, the value and 2^-9
+        r[e] = __builtin_amdgcn_fmed3f(r[e] * 0x1p126f, r[e] * ir, 0x1p-9f);
+      }
+      if (FULL || i < left) {
+        CM[i / 4] = encode4(a);
+        CV[i / 4] = encode4(r);
         if (threadIdx.x % 16 == 0) {
-          t.m_scale[i / kBlock] = am * (1.0f / kFull);
-          t.v_scale[i / kBlock] = ar * (1.0f / kFull);
+          SM[i / kBlock] = am * (1.0f / kFull);
+          SV[i / kBlock] = ar * (1.0f / kFull);
         }
       }
     }
   }
 }
 
+__device__ __forceinline__ int find_tensor(const Args &a, int32_t chunk) {
+  int i = 0;
+  while (i + 1 < a.n && a.chunk_start[i + 1] <= chunk) ++i;
+  return i;
+}
+
 __global__ __launch_bounds__(256) void adamw_update_kernel(Args a, Hypers hy, const Factors *__restrict__ fp) {
   const int k = find_tensor(a, (int32_t)blockIdx.x);
   const Tensor &t = a.t[k];
-  const int64_t lo = (int64_t)((int32_t)blockIdx.x - a.chunk_start[k]) * kChunk, hi = min(t.n, lo + kChunk);
+  const int64_t chunk = (int64_t)((int32_t)blockIdx.x - a.chunk_start[k]) * kChunk;
   const Factors &f = *fp;
   const Hyper &h = hy.g[t.group];
-#define RK_CASE(PD, GD, PT, GT)                           \
-  case (PD) | (GD) << 2:                                  \
-    if (t.m_scale)                                        \
-      update<PT, GT, true>(t, lo, hi, h, f, t.group);     \
-    else                                                  \
-      update<PT, GT, false>(t, lo, hi, h, f, t.group);    \
+  const bool full = chunk + kChunk <= t.n;
+#define RK_CASE(PD, GD, PT, GT)                                   \
+  case (PD) | (GD) << 2:                                          \
+    if (t.m_scale) {                                              \
+      if (full)                                                   \
+        update<PT, GT, true, true>(t, chunk, h, f, t.group);      \
+      else                                                        \
+        update<PT, GT, true, false>(t, chunk, h, f, t.group);     \
+    } else if (full) {                                            \
+      update<PT, GT, false, true>(t, chunk, h, f, t.group);       \
+    } else {                                                      \
+      update<PT, GT, false, false>(t, chunk, h, f, t.group);      \
+    }                                                             \
     break;
   switch (t.kind) {
     RK_CASE(RK_F32, RK_F32, float, float)
@@ -332,8 +377,8 @@ __global__ __launch_bounds__(256) void adamw_update_kernel(Args a, Hypers hy, co
 
 int launches_of(int32_t n_tensors) { return (int)rk::ceil_div(n_tensors, kMaxTensors); }
 
-// workspace: factors, ticket, partial sums
-constexpr size_t kTicketAt = (sizeof(Factors) + 15) / 16 * 16, kPartialAt = kTicketAt + 16;
+// workspace: factors, partial sums
+constexpr size_t kPartialAt = (sizeof(Factors) + 15) / 16 * 16;
 
 }  // namespace
 
@@ -379,16 +424,15 @@ int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors, const 
   RK_CHECK_ARG(chunks < INT32_MAX, "too many elements");
   hipStream_t st = (hipStream_t)stream;
   Factors *f = (Factors *)ws;
-  int32_t *ticket = (int32_t *)((char *)ws + kTicketAt);
   double *partial = (double *)((char *)ws + kPartialAt);
   const bool clip = max_norm > 0.0f;
-  if (!clip) {
-    adamw_begin_kernel<<<1, 64, 0, st>>>(gr, lr, step, f);
-    RK_CHECK_LAUNCH("adamw_begin_kernel");
-  }
   const int launches = launches_of(n_tensors);
+  int32_t n_partial = 0;
   for (int pass = clip ? 0 : 1; pass < 2; ++pass) {
-    int32_t first = 0;
+    if (pass == 1) {
+      adamw_begin_kernel<<<1, 256, 0, st>>>(gr, lr, step, partial, n_partial, max_norm, norm_out, f);
+      RK_CHECK_LAUNCH("adamw_begin_kernel");
+    }
     for (int l = 0; l < launches; ++l) {
       Args a;
       a.n = std::min(kMaxTensors, n_tensors - l * kMaxTensors);
@@ -398,15 +442,14 @@ int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors, const 
         a.t[i] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.n,
                   t.param_dtype | t.grad_dtype << 2, t.group};
         a.chunk_start[i] = c;
-        c += (int32_t)rk::ceil_div(t.n, kChunk);
+        c += (int32_t)rk::ceil_div(t.n, pass == 0 ? kNormChunk : kChunk);
       }
       a.chunk_start[a.n] = c;
       if (pass == 0) {
         const int32_t blocks = std::min(c, kNormBlocks);
-        const int32_t joined = l + 1 == launches ? first + blocks : 0;
-        adamw_norm_kernel<<<blocks, 256, 0, st>>>(a, partial, first, joined, ticket, gr, lr, step, max_norm, norm_out, f);
+        adamw_norm_kernel<<<blocks, 256, 0, st>>>(a, partial + n_partial);
         RK_CHECK_LAUNCH("adamw_norm_kernel");
-        first += blocks;
+        n_partial += blocks;
       } else {
         adamw_update_kernel<<<c, 256, 0, st>>>(a, hy, f);
         RK_CHECK_LAUNCH("adamw_update_kernel");

@@ -172,7 +172,6 @@ _FULL = 448.0       # largest finite e4m3 value
 _TINY = 1e-30       # block maxima below this count as this
 _STATE32 = ("exp_avg", "exp_avg_sq")
 _STATE8 = ("exp_avg8", "exp_avg8_scale", "exp_avg_sq8", "exp_avg_sq8_scale")
-_TENSOR = np.dtype([("ptr", np.uint64, 6), ("n", np.int64), ("kind", np.int32, 4)])     # rk_adamw_tensor
 
 
 def encode_moment(x, keep_above_zero=False):
@@ -195,7 +194,7 @@ def decode_moment(code, scale, like):
 
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (the reference trainer's other choice, train/graph_trainer.py:78-101) with
-    clip_grad_norm_ on the library's two-launch step (rk_adamw_step), over all parameter groups at once.
+    clip_grad_norm_ on the library's fused step (rk_adamw_step), over all parameter groups at once.
 
     Parameters and gradients: contiguous fp32, bfloat16 or fp16 on one HIP device (gradients in the
     parameter's type or fp32); the arithmetic is fp32 and a parameter is rounded once.  Up to
@@ -260,13 +259,13 @@ class FusedAdamW(torch.optim.Optimizer):
         self.lr_dev = torch.zeros(_ffi.ADAMW_MAX_GROUPS, dtype=torch.float32, device=dev)
         self.grad_norm = torch.zeros(1, dtype=torch.float32, device=dev)
 
-    def _check(self, p, g):
-        if not (p.is_cuda and p.dtype in _DTYPES and p.is_contiguous() and g.layout == torch.strided and g.is_contiguous()
-                and (g.dtype == p.dtype or g.dtype == torch.float32)):
-            raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, "FusedAdamW: contiguous fp32, bfloat16 or fp16 parameters on a HIP "
-                               "device with dense gradients of their type or fp32 only")
+    def _refuse(self, p, g):
+        if not p.is_cuda:
+            raise _ffi.RkError(_ffi.RK_ERR_NODEV, "FusedAdamW: parameters on a HIP device only")
         if p.device != self._dev or g.device != self._dev:
             raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, f"FusedAdamW: all parameters on one device ({self._dev})")
+        raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, "FusedAdamW: contiguous fp32, bfloat16 or fp16 parameters on a HIP "
+                           "device with dense gradients of their type or fp32 only")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -274,29 +273,37 @@ class FusedAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        rows, kinds, sizes, dev = [], [], [], self._dev
+        rows, dev, state, strided = [], self._dev, self.state, torch.strided
         for k, group in enumerate(self.param_groups):
             for p in group["params"]:
                 g = p.grad
-                if g is None or not p.numel():
+                if g is None:
+                    continue
+                n = p.numel()
+                if n == 0:
                     continue
                 if dev is None:
                     if not p.is_cuda:
-                        raise _ffi.RkError(_ffi.RK_ERR_NODEV, "FusedAdamW: parameters on a HIP device only")
+                        self._refuse(p, g)
                     self._init_device(p.device)
                     dev = self._dev
-                self._check(p, g)
-                st = self._state_for(p)
-                a, b = (st[x].data_ptr() for x in (_STATE8[::2] if "exp_avg8" in st else _STATE32))
-                sa, sb = (st[x].data_ptr() for x in _STATE8[1::2]) if "exp_avg8" in st else (0, 0)
-                rows.append((p.data_ptr(), g.data_ptr(), a, b, sa, sb))
-                sizes.append(p.numel())
-                kinds.append((_DTYPES[p.dtype], _DTYPES[g.dtype], k, 0))
+                pd, gd = _DTYPES.get(p.dtype), _DTYPES.get(g.dtype)
+                if not (pd is not None and (gd == pd or gd == 0) and g.layout is strided and p.is_contiguous()
+                        and g.is_contiguous() and p.device == dev and g.device == dev):
+                    self._refuse(p, g)
+                st = state[p]
+                if "exp_avg8" not in st and "exp_avg" not in st:
+                    st = self._state_for(p)
+                if "exp_avg8" in st:
+                    rows.append((p.data_ptr(), g.data_ptr(), st["exp_avg8"].data_ptr(), st["exp_avg_sq8"].data_ptr(),
+                                 st["exp_avg8_scale"].data_ptr(), st["exp_avg_sq8_scale"].data_ptr(), n, pd | gd << 32, k))
+                else:
+                    rows.append((p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), 0, 0, n,
+                                 pd | gd << 32, k))
         if not rows:
             return loss
         n = len(rows)
-        table = np.empty(n, _TENSOR)
-        table["ptr"], table["n"], table["kind"] = rows, sizes, kinds
+        table = np.array(rows, np.int64)             # n rows of rk_adamw_tensor (its int32 pairs as one int64 each)
         groups = (_ffi.AdamwGroup * len(self.param_groups))()
         for dst, group in zip(groups, self.param_groups):
             (dst.beta1, dst.beta2), dst.eps, dst.weight_decay = group["betas"], group["eps"], group["weight_decay"]
@@ -305,10 +312,10 @@ class FusedAdamW(torch.optim.Optimizer):
         if self._ws is None or self._ws.numel() * 8 < need:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
-            self._ws = torch.zeros(need // 8, dtype=torch.float64, device=dev)
-        _ffi.call_on(dev, "rk_adamw_step", ptr(table), n, groups, len(groups), ptr(self.step_count), ptr(self.lr_dev),
-                     float(self.max_grad_norm or 0.0), ptr(self.grad_norm), ptr(self._ws), self._ws.numel() * 8,
-                     stream_ptr(dev))
+            self._ws = torch.empty(need // 8, dtype=torch.float64, device=dev)
+        _ffi.call_on(dev, "rk_adamw_step", table.ctypes.data, n, groups, len(groups), self.step_count.data_ptr(),
+                     self.lr_dev.data_ptr(), float(self.max_grad_norm or 0.0), self.grad_norm.data_ptr(),
+                     self._ws.data_ptr(), self._ws.numel() * 8)
         return loss
 
     def sync_lr(self):
