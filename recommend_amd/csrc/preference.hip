@@ -20,6 +20,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / rk::kWave;
+constexpr int kPairThreads = 1024;
+constexpr int kFewRows = 4096;       // rows that one workgroup joins
 
 struct Rows {
   int64_t stride_s, stride_t;   // of the scores, in elements
@@ -40,53 +42,65 @@ __device__ __forceinline__ void merge(float &m, float &s, float om, float os) {
   m = nm;
 }
 
+// One part of one row: its (max, sum) and, if the row's item lies in it, the item's score.  The next step's
+// vectors are on their way while a step's exponentials are computed.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__restrict__ x, float2 *__restrict__ part,
-                                                            int32_t *__restrict__ ticket) {
-  constexpr int VEC = rk::Elem<T>::kVec, U = 4;
+                                                            float *__restrict__ score) {
+  constexpr int VEC = rk::Elem<T>::kVec, U = 4, kStep = U * kThreads * VEC;
   __shared__ float s_m[kWaves], s_s[kWaves];
-  if (blockIdx.x == 0 && threadIdx.x == 0) ticket[0] = 0;   // for the closing launch
   const int64_t row = blockIdx.x / a.parts;
   const int32_t p = (int32_t)(blockIdx.x - row * a.parts), s = (int32_t)(row / a.T), t = (int32_t)(row - (int64_t)s * a.T);
-  if (a.items[s * a.ld_items + t] == a.ignore) return;
+  const int64_t y = a.items[s * a.ld_items + t];
+  if (y == a.ignore) return;
   const int32_t lo = p * a.part_len, hi = min(a.V, lo + a.part_len);
   const T *r = x + s * a.stride_s + t * a.stride_t;
+  if (threadIdx.x == 0) {
+    if (y >= lo && y < hi)
+      score[row] = rk::Elem<T>::get(r[y]);
+    else if (p == 0 && (y < 0 || y >= a.V))
+      score[row] = __builtin_nanf("");   // an item outside the catalogue has no score
+  }
   float m = -__FLT_MAX__, sum = 0.0f;
-  int32_t j = lo + (int32_t)threadIdx.x * VEC;
-  for (; j + (U - 1) * kThreads * VEC + VEC <= hi; j += U * kThreads * VEC) {
-    rk::Pack<T, VEC> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u].load(r + j + u * kThreads * VEC);
-    float f[U][VEC], top = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u].widen(f[u]);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[u][e]);
-    }
+  auto add = [&](const float *f, int n) {
+    float top = m;
+    for (int e = 0; e < n; ++e) top = fmaxf(top, f[e]);
     sum *= __expf(m - top);
     m = top;
+    for (int e = 0; e < n; ++e) sum += __expf(f[e] - m);
+  };
+  const int32_t steps = (hi - lo) / kStep;
+  const T *q = r + lo + (int)threadIdx.x * VEC;
+  rk::Pack<T, VEC> v[U];
+  if (steps > 0)
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) v[u].load(q + u * kThreads * VEC);
+  for (int32_t k = 0; k < steps; ++k) {
+    float f[U * VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum += __expf(f[u][e] - m);
+    for (int u = 0; u < U; ++u) v[u].widen(*reinterpret_cast<float(*)[VEC]>(f + u * VEC));
+    q += kStep;
+    if (k + 1 < steps)
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].load(q + u * kThreads * VEC);
+    add(f, U * VEC);
   }
-  for (; j < hi; j += kThreads * VEC) {
-    float f[VEC], top = m;
+  // the rest of the part: less than one step
+  int32_t j = lo + steps * kStep + (int32_t)threadIdx.x * VEC;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (j + u * kThreads * VEC + VEC <= hi) v[u].load(r + j + u * kThreads * VEC);
+#pragma unroll
+  for (int u = 0; u < U; ++u, j += kThreads * VEC) {
+    float f[VEC];
     if (j + VEC <= hi) {
-      rk::Pack<T, VEC> v;
-      v.load(r + j);
-      v.widen(f);
-    } else {
+      v[u].widen(f);
+      add(f, VEC);
+    } else if (j < hi) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = j + e < hi ? rk::Elem<T>::get(r[j + e]) : neg_inf();
+      add(f, VEC);
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e]);
-    sum *= __expf(m - top);
-    m = top;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sum += __expf(f[e] - m);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
@@ -105,26 +119,32 @@ __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__r
   }
 }
 
-// one wavefront: the log-probability of list s; leaves (max, log sum) of its rows in stat
-template <typename T>
-__device__ __forceinline__ float list_logp(const Rows &a, const T *__restrict__ x, const float2 *__restrict__ part,
-                                           float2 *__restrict__ stat, int32_t s, int average, int32_t &used) {
-  const int lane = threadIdx.x % rk::kWave;
+// log-probability of the row's item from the row's parts, which it joins in order; leaves (max, log sum)
+__device__ __forceinline__ float row_logp(const Rows &a, int64_t row, const float2 *__restrict__ part,
+                                          const float *__restrict__ score, float2 *__restrict__ stat) {
+  float m = -__FLT_MAX__, q = 0.0f;
+#pragma unroll 4
+  for (int p = 0; p < a.parts; ++p) {
+    const float2 o = part[row * a.parts + p];
+    merge(m, q, o.x, o.y);
+  }
+  const float lq = logf(q);
+  stat[row] = make_float2(m, lq);
+  return (score[row] - m) - lq;
+}
+
+// One wavefront for every list: its log-probability and the number of its places in use.
+__global__ __launch_bounds__(kThreads) void lists_kernel(Rows a, const float2 *__restrict__ part,
+                                                         const float *__restrict__ score, float2 *__restrict__ stat,
+                                                         int average, float *__restrict__ logps,
+                                                         int32_t *__restrict__ used) {
+  const int32_t s = (int32_t)blockIdx.x * kWaves + threadIdx.x / rk::kWave;
+  if (s >= a.S) return;
   double sum = 0.0;
   int32_t n = 0;
-  for (int32_t t = lane; t < a.T; t += rk::kWave) {
-    const int64_t y = a.items[s * a.ld_items + t], row = (int64_t)s * a.T + t;
-    if (y == a.ignore) continue;
-    float m = -__FLT_MAX__, q = 0.0f;
-    for (int p = 0; p < a.parts; ++p) {
-      const float2 o = part[row * a.parts + p];
-      merge(m, q, o.x, o.y);
-    }
-    const float lq = logf(q);
-    stat[row] = make_float2(m, lq);
-    // an item outside the catalogue has no score: its log-probability is not a number
-    const float xy = y >= 0 && y < a.V ? rk::Elem<T>::get(x[s * a.stride_s + t * a.stride_t + y]) : __builtin_nanf("");
-    sum += (double)((xy - m) - lq);
+  for (int32_t t = threadIdx.x % rk::kWave; t < a.T; t += rk::kWave) {
+    if (a.items[s * a.ld_items + t] == a.ignore) continue;
+    sum += (double)row_logp(a, (int64_t)s * a.T + t, part, score, stat);
     ++n;
   }
 #pragma unroll
@@ -132,20 +152,8 @@ __device__ __forceinline__ float list_logp(const Rows &a, const T *__restrict__ 
     sum += __shfl_xor(sum, off, rk::kWave);
     n += __shfl_xor(n, off, rk::kWave);
   }
-  used = n;
-  return (float)(average && n > 0 ? sum / n : sum);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void lists_kernel(Rows a, const T *__restrict__ x, const float2 *__restrict__ part,
-                                                         float2 *__restrict__ stat, int average, float *__restrict__ logps,
-                                                         int32_t *__restrict__ used) {
-  const int32_t s = (int32_t)blockIdx.x * kWaves + threadIdx.x / rk::kWave;
-  if (s >= a.S) return;
-  int32_t n;
-  const float v = list_logp(a, x, part, stat, s, average, n);
   if (threadIdx.x % rk::kWave == 0) {
-    logps[s] = v;
+    logps[s] = (float)(average && n > 0 ? sum / n : sum);
     used[s] = n;
   }
 }
@@ -176,76 +184,101 @@ __device__ __forceinline__ float pair_term(float d, float beta, float eps, int k
   return term;
 }
 
-// Pairs p and P + p, one wavefront each; the workgroup that finishes last adds the pairs' terms in
-// order.  Every pair's term reaches memory by an agent-scope store in front of its ticket and is read
-// back by an agent-scope load behind the last ticket: the workgroups run under different L2 caches.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void pairs_kernel(Rows a, const T *__restrict__ x, const float2 *__restrict__ part,
-                                                         float2 *__restrict__ stat, const float *__restrict__ ref,
-                                                         int average, float beta, float eps, int kind,
-                                                         float *__restrict__ logps, int32_t *__restrict__ used,
-                                                         float *__restrict__ slope_out, float *__restrict__ terms,
-                                                         int32_t *__restrict__ ticket, float *__restrict__ loss) {
-  __shared__ int s_last;
-  __shared__ double s_sum[kWaves];
-  const int lane = threadIdx.x % rk::kWave;
-  const int32_t P = a.S / 2, p = (int32_t)blockIdx.x * kWaves + threadIdx.x / rk::kWave;
-  if (p < P) {
-    int32_t nc, nr;
-    const float c = list_logp(a, x, part, stat, p, average, nc);
-    const float r = list_logp(a, x, part, stat, P + p, average, nr);
-    if (lane == 0) {
-      float slope;
-      const float term = pair_term((c - ref[p]) - (r - ref[P + p]), beta, eps, kind, slope);
-      logps[p] = c;
-      logps[P + p] = r;
-      used[p] = nc;
-      used[P + p] = nr;
-      slope_out[p] = slope / (float)P;
-      slope_out[P + p] = -slope / (float)P;
-      __hip_atomic_store(&terms[p], term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// One workgroup: the pairs' terms, their slopes and the mean, added in a fixed order.  ROWS: it also forms the
+// lists' log-probabilities, from up to kFewRows rows, a thread for each (one launch instead of two).
+template <bool ROWS>
+__global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float2 *__restrict__ part,
+                                                             const float *__restrict__ score, float2 *__restrict__ stat,
+                                                             const float *__restrict__ ref, int average, float beta,
+                                                             float eps, int kind, float *__restrict__ logps,
+                                                             int32_t *__restrict__ used, float *__restrict__ slope_out,
+                                                             float *__restrict__ loss) {
+  __shared__ float s_row[ROWS ? kFewRows : 1], s_logp[ROWS ? kFewRows : 1];
+  __shared__ double s_sum[kPairThreads / rk::kWave];
+  const int32_t P = a.S / 2;
+  if constexpr (ROWS) {
+    const int32_t rows = a.S * a.T;
+    for (int32_t row = threadIdx.x; row < rows; row += kPairThreads) {
+      const int32_t s = row / a.T, t = row - s * a.T;
+      const bool in = a.items[s * a.ld_items + t] != a.ignore;
+      // a place that is not in use is marked by the one value that no log-probability has
+      s_row[row] = in ? row_logp(a, row, part, score, stat) : __builtin_inff();
     }
+    __syncthreads();
+    // 16 lanes for every list
+    const int sub = threadIdx.x % 16;
+    for (int32_t s0 = 0; s0 < a.S; s0 += kPairThreads / 16) {
+      const int32_t s = s0 + (int32_t)threadIdx.x / 16;
+      double sum = 0.0;
+      int32_t n = 0;
+      if (s < a.S)
+        for (int32_t t = sub; t < a.T; t += 16) {
+          const float v = s_row[s * a.T + t];
+          if (v == __builtin_inff()) continue;
+          sum += (double)v;
+          ++n;
+        }
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) {
+        sum += __shfl_xor(sum, off, 16);
+        n += __shfl_xor(n, off, 16);
+      }
+      if (s < a.S && sub == 0) {
+        const float v = (float)(average && n > 0 ? sum / n : sum);
+        s_logp[s] = logps[s] = v;
+        used[s] = n;
+      }
+    }
+    __syncthreads();
   }
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0)
-    s_last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)gridDim.x - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
   double sum = 0.0;
-  for (int32_t i = threadIdx.x; i < P; i += kThreads)
-    sum += (double)__hip_atomic_load(&terms[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int32_t p = threadIdx.x; p < P; p += kPairThreads) {
+    const float c = ROWS ? s_logp[p] : logps[p], r = ROWS ? s_logp[P + p] : logps[P + p];
+    float slope;
+    sum += (double)pair_term((c - ref[p]) - (r - ref[P + p]), beta, eps, kind, slope);
+    slope_out[p] = slope / (float)P;
+    slope_out[P + p] = -slope / (float)P;
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, rk::kWave);
-  if (lane == 0) s_sum[threadIdx.x / rk::kWave] = sum;
+  if (threadIdx.x % rk::kWave == 0) s_sum[threadIdx.x / rk::kWave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     double all = s_sum[0];
-    for (int w = 1; w < kWaves; ++w) all += s_sum[w];
+    for (int w = 1; w < kPairThreads / rk::kWave; ++w) all += s_sum[w];
     loss[0] = (float)(all / P);
   }
 }
 
-// dx = c * ([j = y] - exp((x - max) - log sum)), c = (g_loss * slope + g_logps) of the row's list
-template <typename T>
+// dx = c * ([j = y] - exp((x - max) - log sum)), c = (g_loss * slope + g_logps) of the row's list.  From the
+// last row to the first: those were read last and some of them are still cached.  ONCE: a gradient that
+// is larger than what the caches should hold is stored past them (left there, its 403 MB were written
+// back under the next call's forward launch, which took 74 us instead of 41).
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__restrict__ x, const float2 *__restrict__ stat,
                                                             const float *__restrict__ g_loss, const float *__restrict__ slope,
                                                             const float *__restrict__ g_logps, int average,
                                                             const int32_t *__restrict__ used, T *__restrict__ dx) {
   constexpr int VEC = rk::Elem<T>::kVec, U = 4;
-  const int64_t row = blockIdx.x / a.parts;
-  const int32_t p = (int32_t)(blockIdx.x - row * a.parts), s = (int32_t)(row / a.T), t = (int32_t)(row - (int64_t)s * a.T);
+  const uint32_t block = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = block / a.parts;
+  const int32_t p = (int32_t)(block - row * a.parts), s = (int32_t)(row / a.T), t = (int32_t)(row - (int64_t)s * a.T);
   const int32_t lo = p * a.part_len, hi = min(a.V, lo + a.part_len);
   const int64_t y = a.items[s * a.ld_items + t];
   T *d = dx + row * a.V;
+  auto put = [&](const rk::Pack<T, VEC> &o, int32_t j) {
+    if constexpr (ONCE)
+      o.store_once(d + j);
+    else
+      o.store(d + j);
+  };
   if (y == a.ignore) {
     rk::Pack<T, VEC> zero;
 #pragma unroll
     for (int i = 0; i < rk::Pack<T, VEC>::kWords; ++i) zero.w[i] = 0u;
     for (int32_t j = lo + (int32_t)threadIdx.x * VEC; j < hi; j += kThreads * VEC) {
       if (j + VEC <= hi) {
-        zero.store(d + j);
+        put(zero, j);
       } else {
         for (int e = 0; e < VEC && j + e < hi; ++e) d[j + e] = rk::Elem<T>::put(0.0f);
       }
@@ -270,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__r
     }
     rk::Pack<T, VEC> o;
     o.narrow(f);
-    o.store(d + j);
+    put(o, j);
   };
   int32_t j = lo + (int32_t)threadIdx.x * VEC;
   for (; j + (U - 1) * kThreads * VEC + VEC <= hi; j += U * kThreads * VEC) {
@@ -295,17 +328,20 @@ __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__r
   }
 }
 
-// parts of a row: enough workgroups for the GPU, parts of at least kMinPart scores
-constexpr int kMinPart = 4096, kWantBlocks = 2048;
-void cut(Rows &a) {
+// Parts of a row, of at least kMinPart scores: enough workgroups for the GPU, and short ones, whose ends
+// do not leave CUs idle (3200 rows of 63001 scores in bf16, 1600 of them in use: forward 41 us with
+// 2048 workgroups wanted, 35 with 8192, above that the joining of the parts takes what it gains;
+// backward 119 us with 4096, 95 with 32768, 84 with 65536, 89 with parts of 2048).
+constexpr int kMinPart = 4096, kWantFwd = 8192, kWantBwd = 65536;
+void cut(Rows &a, int want_blocks) {
   const int64_t rows = (int64_t)a.S * a.T;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(rk::ceil_div(kWantBlocks, rows), rk::ceil_div(a.V, kMinPart)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(rk::ceil_div(want_blocks, rows), rk::ceil_div(a.V, kMinPart)));
   a.part_len = (int32_t)(rk::ceil_div(rk::ceil_div(a.V, want), 8) * 8);
   a.parts = (int32_t)rk::ceil_div(a.V, a.part_len);
 }
 
 int make_rows(Rows &a, int32_t dtype, int32_t S, int32_t T, int32_t V, int64_t stride_s, int64_t stride_t,
-              const int64_t *items, int64_t ld_items, int64_t ignore) {
+              const int64_t *items, int64_t ld_items, int64_t ignore, int want_blocks) {
   RK_CHECK_ARG(dtype == RK_F32 || dtype == RK_BF16 || dtype == RK_F16, "unknown element type %d", dtype);
   RK_CHECK_ARG(S >= 0 && T >= 0 && V >= 1, "bad size: %d lists, %d places, %d items", S, T, V);
   // a part's last step may look a few thousand scores past its end before it stops
@@ -313,28 +349,35 @@ int make_rows(Rows &a, int32_t dtype, int32_t S, int32_t T, int32_t V, int64_t s
   a = {stride_s, stride_t, S, T, V, 0, 0, items, ld_items, ignore};
   if (S == 0 || T == 0) return RK_OK;
   RK_CHECK_ARG(items, "null pointer");
-  cut(a);
+  cut(a, want_blocks);
   RK_CHECK_ARG((int64_t)S * T * a.parts < INT32_MAX, "too many rows");
   return RK_OK;
 }
 
-struct Ws {   // of the forward calls, in 4-byte words: parts' (max, sum), pairs' terms, ticket
-  int64_t part, terms, ticket, words;
+struct Ws {   // of the forward calls, in 4-byte words: parts' (max, sum), the items' scores
+  int64_t part, score, words;
 };
 Ws ws_of(const Rows &a) {
   Ws w;
   w.part = 0;
-  w.terms = 2 * (int64_t)a.S * a.T * a.parts;
-  w.ticket = w.terms + a.S;
-  w.words = w.ticket + 4;
+  w.score = 2 * (int64_t)a.S * a.T * a.parts;
+  w.words = w.score + (int64_t)a.S * a.T;
   return w;
 }
 
 template <typename T>
 int launch_rows_fwd(const Rows &a, const void *x, float *ws, const Ws &w, hipStream_t st) {
-  rows_fwd_kernel<T><<<(uint32_t)((int64_t)a.S * a.T * a.parts), kThreads, 0, st>>>(
-      a, (const T *)x, (float2 *)(ws + w.part), (int32_t *)(ws + w.ticket));
+  rows_fwd_kernel<T><<<(uint32_t)((int64_t)a.S * a.T * a.parts), kThreads, 0, st>>>(a, (const T *)x, (float2 *)(ws + w.part),
+                                                                                  ws + w.score);
   RK_CHECK_LAUNCH("rows_fwd_kernel");
+  return RK_OK;
+}
+
+int launch_lists(const Rows &a, int average, float *stat, float *logps, int32_t *used, const float *ws, const Ws &w,
+                 hipStream_t st) {
+  lists_kernel<<<(uint32_t)rk::ceil_div(a.S, kWaves), kThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score,
+                                                                        (float2 *)stat, average, logps, used);
+  RK_CHECK_LAUNCH("lists_kernel");
   return RK_OK;
 }
 
@@ -343,10 +386,7 @@ int run_lists(const Rows &a, const void *x, int average, float *stat, float *log
               hipStream_t st) {
   const Ws w = ws_of(a);
   if (int rc = launch_rows_fwd<T>(a, x, ws, w, st)) return rc;
-  lists_kernel<T><<<(uint32_t)rk::ceil_div(a.S, kWaves), kThreads, 0, st>>>(a, (const T *)x, (const float2 *)(ws + w.part),
-                                                                          (float2 *)stat, average, logps, used);
-  RK_CHECK_LAUNCH("lists_kernel");
-  return RK_OK;
+  return launch_lists(a, average, stat, logps, used, ws, w, st);
 }
 
 template <typename T>
@@ -354,18 +394,31 @@ int run_pairs(const Rows &a, const void *x, const float *ref, int average, float
               float *logps, int32_t *used, float *slope, float *loss, float *ws, hipStream_t st) {
   const Ws w = ws_of(a);
   if (int rc = launch_rows_fwd<T>(a, x, ws, w, st)) return rc;
-  pairs_kernel<T><<<(uint32_t)rk::ceil_div(a.S / 2, kWaves), kThreads, 0, st>>>(
-      a, (const T *)x, (const float2 *)(ws + w.part), (float2 *)stat, ref, average, beta, eps, kind, logps, used, slope,
-      ws + w.terms, (int32_t *)(ws + w.ticket), loss);
+  const float2 *part = (const float2 *)(ws + w.part);
+  if ((int64_t)a.S * a.T <= kFewRows) {
+    pairs_kernel<true><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind, logps,
+                                                  used, slope, loss);
+  } else {
+    if (int rc = launch_lists(a, average, stat, logps, used, ws, w, st)) return rc;
+    pairs_kernel<false><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind,
+                                                   logps, used, slope, loss);
+  }
   RK_CHECK_LAUNCH("pairs_kernel");
   return RK_OK;
 }
 
+constexpr int64_t kStreamBytes = 64 << 20;   // gradients from this size on are stored past the caches
+
 template <typename T>
 int run_bwd(const Rows &a, const void *x, const float *stat, const float *g_loss, const float *slope, const float *g_logps,
             int average, const int32_t *used, void *dx, hipStream_t st) {
-  rows_bwd_kernel<T><<<(uint32_t)((int64_t)a.S * a.T * a.parts), kThreads, 0, st>>>(
-      a, (const T *)x, (const float2 *)stat, g_loss, slope, g_logps, average, used, (T *)dx);
+  const uint32_t blocks = (uint32_t)((int64_t)a.S * a.T * a.parts);
+  if ((int64_t)a.S * a.T * a.V * (int64_t)sizeof(T) >= kStreamBytes)
+    rows_bwd_kernel<T, true><<<blocks, kThreads, 0, st>>>(a, (const T *)x, (const float2 *)stat, g_loss, slope, g_logps, average,
+                                                        used, (T *)dx);
+  else
+    rows_bwd_kernel<T, false><<<blocks, kThreads, 0, st>>>(a, (const T *)x, (const float2 *)stat, g_loss, slope, g_logps,
+                                                         average, used, (T *)dx);
   RK_CHECK_LAUNCH("rows_bwd_kernel");
   return RK_OK;
 }
@@ -377,7 +430,7 @@ extern "C" {
 size_t rk_list_logps_ws_bytes(int32_t S, int32_t T, int32_t V) {
   if (S <= 0 || T <= 0 || V <= 0) return 0;
   Rows a = {0, 0, S, T, V, 0, 0, nullptr, 0, 0};
-  cut(a);
+  cut(a, kWantFwd);
   return (size_t)ws_of(a).words * 4;
 }
 
@@ -389,7 +442,7 @@ int rk_list_logps_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
                       int64_t stride_t, const int64_t *items, int64_t ld_items, int64_t ignore_index, int32_t average,
                       float *stat, float *logps, int32_t *used, void *ws, size_t ws_bytes, void *stream) {
   Rows a;
-  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index)) return rc;
+  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index, kWantFwd)) return rc;
   RK_CHECK_ARG(S == 0 || T > 0, "lists without places");
   if (S == 0) return RK_OK;
   RK_CHECK_ARG(scores && stat && logps && used && ws, "null pointer");
@@ -402,7 +455,7 @@ int rk_preference_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
                       const float *ref_logps, float beta, float label_smoothing, int32_t kind, float *stat, float *logps,
                       int32_t *used, float *slope, float *loss, void *ws, size_t ws_bytes, void *stream) {
   Rows a;
-  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index)) return rc;
+  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index, kWantFwd)) return rc;
   RK_CHECK_ARG(S >= 2 && S % 2 == 0 && T > 0, "pairs of lists are needed: %d lists of %d places", S, T);
   RK_CHECK_ARG(kind == RK_PREF_SIGMOID || kind == RK_PREF_HINGE || kind == RK_PREF_SQUARED, "unknown kind %d", kind);
   RK_CHECK_ARG(beta > 0.0f, "beta must be positive");
@@ -419,7 +472,7 @@ int rk_list_logps_bwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
                       const float *stat, const int32_t *used, const float *g_loss, const float *slope,
                       const float *g_logps, void *d_scores, void *stream) {
   Rows a;
-  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index)) return rc;
+  if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index, kWantBwd)) return rc;
   if (S == 0 || T == 0) return RK_OK;
   RK_CHECK_ARG(scores && stat && used && d_scores, "null pointer");
   RK_CHECK_ARG(!g_loss || slope, "the gradient of the loss needs the slopes of rk_preference_fwd");
