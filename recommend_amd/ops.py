@@ -408,6 +408,7 @@ def bpr_gather_dot_sampled(U, I, users, pos, neg_rank, pos_ptr, pos_items, mask=
 # --------------------------------------------------------------------------
 # embedding lookup with scaling; log-probabilities of item lists
 # --------------------------------------------------------------------------
+_MAX_INT = 2 ** 31 - 2 ** 24     # sizes are int32 at the C boundary
 _ELEM = {torch.float32: _ffi.F32, torch.bfloat16: _ffi.BF16, torch.float16: _ffi.F16}
 
 
@@ -439,6 +440,19 @@ def _once(backward):
     def run(ctx, *grads):
         return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
+
+
+class _NoSecondDerivative(torch.autograd.Function):
+    """The identity on a gradient that depends on saved inputs (once_differentiable takes it for a constant where
+    the upstream gradient is one): differentiating it raises."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise RuntimeError("the list operators are differentiable once: they have no second derivative")
 
 
 class _EmbeddingLookup(torch.autograd.Function):
@@ -486,6 +500,8 @@ def embedding_lookup(weight, ids, scale=1.0, padding_idx=None):
         raise ValueError(f"embedding_lookup: the table is [rows, D], got {tuple(weight.shape)}")
     if weight.dtype not in _ELEM:
         _elem(weight, "embedding_lookup")
+    if max(weight.shape) >= _MAX_INT:
+        raise ValueError(f"embedding_lookup: a table of {tuple(weight.shape)} has more than 2^31 rows or columns")
     if ids.dtype != torch.int64 and ids.dtype != torch.int32:
         raise ValueError(f"embedding_lookup: ids are int32 or int64, not {ids.dtype}")
     if padding_idx is None:
@@ -516,6 +532,8 @@ def _list_args(scores, items, what):
                          f"got {tuple(scores.shape)} and {tuple(items.shape)}")
     if 0 in scores.shape[1:]:
         raise ValueError(f"{what}: no places or no catalogue in {tuple(scores.shape)}")
+    if max(scores.shape) >= _MAX_INT:
+        raise ValueError(f"{what}: more than 2^31 lists, places or items in {tuple(scores.shape)}")
     _same_device(scores, items)
     return items.to(torch.int64).contiguous()
 
@@ -563,8 +581,15 @@ class _ListLogps(torch.autograd.Function):
         return logps, loss
 
     @staticmethod
-    @_once
     def backward(ctx, g_logps, g_loss=None):
+        if not torch.is_grad_enabled():
+            return _ListLogps._gradients(ctx, g_logps, g_loss)
+        with torch.no_grad():
+            dx = _ListLogps._gradients(ctx, g_logps, g_loss)[0]
+        return (None if dx is None else _NoSecondDerivative.apply(dx.requires_grad_(True))), None, None, None
+
+    @staticmethod
+    def _gradients(ctx, g_logps, g_loss):
         scores, items, keep = ctx.saved_tensors
         ignore_index, average, pairs = ctx.args
         if g_logps is None and g_loss is None:

@@ -233,7 +233,14 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError("FusedAdamW: betas in [0, 1), eps, weight_decay and lr not negative")
 
     def __getstate__(self):
-        return {**super().__getstate__(), "_ws": None}
+        steps = int(self.step_count.item()) if self._dev is not None else self._restored_step
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "state_bits": self.state_bits,
+                "min_8bit_size": self.min_8bit_size, "_restored_step": steps}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_dev" not in self.__dict__:      # a copy or an unpickled optimizer: device scalars are made anew
+            self._dev = self._rates = self._ws = self.grad_norm = None
 
     def _is8(self, p):
         return self.state_bits == 8 and p.numel() >= self.min_8bit_size

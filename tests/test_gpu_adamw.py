@@ -242,6 +242,23 @@ def test_checkpoints_of_other_forms_load():
 
 
 @pytest.mark.parametrize("bits", [8, 32])
+def test_copies_continue(bits):
+    g = torch.Generator().manual_seed(12)
+    p = params_of([(100, 64)], g)[0]
+    opt = FusedAdamW([p], lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+    grads = [torch.randn(100, 64, generator=g).to(DEV) for _ in range(3)]
+    p.grad = grads[0]
+    opt.step()
+    q, other = copy.deepcopy((p, opt))
+    assert other.param_groups[0]["params"][0] is q
+    for x in grads[1:]:
+        p.grad, q.grad = x, x.clone()
+        opt.step()
+        other.step()
+    assert torch.equal(p, q) and int(other.step_count) == 3
+
+
+@pytest.mark.parametrize("bits", [8, 32])
 def test_recorded_in_a_graph_and_replayed(bits):
     g = torch.Generator().manual_seed(13)
     ours = params_of([(100, 64), (64,)], g)

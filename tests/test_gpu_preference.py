@@ -254,7 +254,8 @@ def test_recorded_in_a_graph_and_replayed_beside_eager_work():
 
     def step():
         loss, logps = preference_loss(scores, items, ref)
-        return loss, logps, torch.autograd.grad(loss, scores)[0]
+        dx, = torch.autograd.grad(loss, scores)
+        return loss.detach(), logps.detach(), dx
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
