@@ -6,6 +6,8 @@
 // lane groups add them in registers in that order and write each row of dW once.  The sums are fp32
 // whatever the tensors' type, the same bits on every run, and rounded once.
 //
+// Up to kFewIds ids one launch does all of it (512 ids of width 64, 7050 rows: 12 us; the three launches
+// below 3 + 5 + 4 and the gaps between them, and two launches more for the host).  Otherwise:
 // Sort: up to kRankSortMax ids one launch counts, for every id, the ids that come before it.  More
 // ids take an LSD radix sort with digits of up to 9 bits: per digit one launch that counts every
 // tile's digits, one that adds up each digit's counts over the tiles and one that places the ids.
@@ -29,6 +31,8 @@ constexpr int kSortWaves = kSortThreads / rk::kWave;
 constexpr int kMaxDigitBits = 9;      // one thread for each digit
 constexpr int kTileSteps = 8;         // ids of a thread: they stay in registers
 constexpr int kTile = kSortThreads * kTileSteps;
+constexpr int kFewBits = 9, kFewIds = 1 << kFewBits;   // ids that every summing workgroup sorts itself: one launch
+constexpr int32_t kFewRows = 1 << (32 - kFewBits);      // (key and position have to fit a word)
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
 constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
 constexpr int kPerGroup = 16;         // sorted entries of a lane group
@@ -299,24 +303,19 @@ __device__ __forceinline__ int32_t lower_bound(const int32_t *__restrict__ keys,
   return lo;
 }
 
+// zeros in row z * kZeroRows + threadIdx.x where `absent` says so, a wavefront's 64 rows together
 template <typename T, int VEC>
-__device__ __forceinline__ void zero_rows(const SumArgs &a, int32_t z, T *__restrict__ dW) {
-  const int32_t v = z * kZeroRows + (int32_t)threadIdx.x;
-  bool absent = false;
-  if (v < a.rows) {
-    const int32_t at = lower_bound(a.keys, a.n, v);
-    absent = !(at < a.n && a.keys[at] == v);
-  }
+__device__ __forceinline__ void zero_rows(int32_t z, bool absent, int32_t D, T *__restrict__ dW) {
   const uint64_t mask = __ballot(absent);
   if (!mask) return;
-  const int lane = threadIdx.x % rk::kWave, per_row = (a.D + VEC - 1) / VEC;
+  const int lane = threadIdx.x % rk::kWave, per_row = (D + VEC - 1) / VEC;
   const int64_t row0 = (int64_t)z * kZeroRows + (threadIdx.x - lane);
   rk::Pack<T, VEC> zero;
 #pragma unroll
   for (int i = 0; i < rk::Pack<T, VEC>::kWords; ++i) zero.w[i] = 0u;
   for (int i = lane; i < rk::kWave * per_row; i += rk::kWave) {
     const int r = i / per_row;
-    if ((mask >> r) & 1) zero.store(dW + (row0 + r) * a.D + min((i - r * per_row) * VEC, a.D - VEC));
+    if ((mask >> r) & 1) zero.store(dW + (row0 + r) * D + min((i - r * per_row) * VEC, D - VEC));
   }
 }
 
@@ -330,35 +329,20 @@ __device__ __forceinline__ void put_row(T *__restrict__ dst, const float (&acc)[
   v.store(dst);
 }
 
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__restrict__ g, T *__restrict__ dW) {
+// Adds a workgroup's `count` sorted entries: key[1 ..] and pos[0 ..], with the key in front of them in key[0]
+// and the one behind them in key[1 + count].  pieces: where the parts of rows go that begin in front of
+// them or go on behind them (ALONE: none does).
+template <typename T, int VEC, bool ALONE>
+__device__ __forceinline__ void sum_entries(const SumArgs &a, const T *__restrict__ g, T *__restrict__ dW,
+                                            const int32_t *key, const int32_t *pos, int count, int per_group,
+                                            float *__restrict__ pieces) {
   constexpr int U = 8;                                   // rows of g in flight per lane group
-  __shared__ int32_t s_key[kMaxEntries + 2];             // [0]: the key in front, [1 + count]: the key behind
-  __shared__ int32_t s_pos[kMaxEntries];
   __shared__ float s_head[256 * VEC], s_tail[256 * VEC]; // what a group has of the row it begins / ends in
   __shared__ uint8_t s_through[256], s_has_tail[256];
-  if ((int32_t)blockIdx.x >= a.blocks) {
-    zero_rows<T, VEC>(a, (int32_t)blockIdx.x - a.blocks, dW);
-    return;
-  }
-  const int per_block = a.G * a.per_group;
-  const int32_t s0 = (int32_t)blockIdx.x * per_block, s1 = (int32_t)min((int64_t)a.n, (int64_t)s0 + per_block);
-  int count = s1 - s0;
-  for (int i = threadIdx.x; i < count; i += 256) {
-    s_key[1 + i] = a.keys[s0 + i];
-    s_pos[i] = a.perm[s0 + i];
-  }
-  if (threadIdx.x == 0) {
-    s_key[0] = s0 > 0 ? a.keys[s0 - 1] : -1;
-    s_key[1 + count] = s1 < a.n ? a.keys[s1] : -1;
-  }
-  __syncthreads();
-  if (s_key[count] >= a.rows) count = lower_bound(s_key + 1, count, a.rows);   // entries that add nothing come last
-  if (count == 0) return;
   const int grp = threadIdx.x / a.L, l = threadIdx.x - grp * a.L;
-  const int es = min(count, grp * a.per_group), ee = min(count, es + a.per_group);
+  const int es = min(count, grp * per_group), ee = min(count, es + per_group);
   const bool live = grp < a.G && es < ee;
-  const bool began_before = live && s_key[es] == s_key[1 + es];
+  const bool began_before = live && key[es] == key[1 + es];
 
   for (int c0 = 0; c0 < a.D; c0 += a.L * VEC) {
     const bool on = live && c0 + l * VEC < a.D;
@@ -368,16 +352,16 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
       float acc[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[e] = 0.0f;
-      int32_t cur = s_key[1 + es];
+      int32_t cur = key[1 + es];
       bool first = began_before;                         // still in the row that an earlier group began
       for (int i = es; i < ee; i += U) {
         rk::Pack<T, VEC> v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) v[j].load_once(g + (int64_t)s_pos[min(i + j, ee - 1)] * a.D + col);
+        for (int j = 0; j < U; ++j) v[j].load_once(g + (int64_t)pos[min(i + j, ee - 1)] * a.D + col);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
           if (i + j >= ee) break;
-          const int32_t k = s_key[1 + i + j];
+          const int32_t k = key[1 + i + j];
           if (k != cur) {
             if (first) {
 #pragma unroll
@@ -396,7 +380,7 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
           for (int e = 0; e < VEC; ++e) acc[e] += x[e];
         }
       }
-      const bool goes_on = s_key[1 + ee] == cur;
+      const bool goes_on = key[1 + ee] == cur;
       if (first) {
         through = goes_on;
 #pragma unroll
@@ -425,15 +409,15 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
         for (int e = 0; e < VEC; ++e) acc[e] += s_head[(j * a.L + l) * VEC + e];
         open = s_through[j];
       }
-      if (!open) {
-        put_row<T, VEC>(dW + (int64_t)s_key[ee] * a.D + col, acc, a.scale);
-      } else {
-        float *p = a.pieces + ((int64_t)blockIdx.x * 2 + 1) * a.D + col;
+      if (ALONE || !open) {
+        put_row<T, VEC>(dW + (int64_t)key[ee] * a.D + col, acc, a.scale);
+      } else if constexpr (!ALONE) {
+        float *p = pieces + a.D + col;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) p[e] = acc[e];
       }
     }
-    if (on && grp == 0 && began_before) {                // the row that an earlier workgroup began
+    if (!ALONE && on && grp == 0 && began_before) {      // the row that an earlier workgroup began
       float acc[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[e] = s_head[slot + e];
@@ -441,12 +425,98 @@ __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__rest
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] += s_head[((j + 1) * a.L + l) * VEC + e];
       }
-      float *p = a.pieces + (int64_t)blockIdx.x * 2 * a.D + col;
+      float *p = pieces + col;
 #pragma unroll
       for (int e = 0; e < VEC; ++e) p[e] = acc[e];
     }
     __syncthreads();
   }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__restrict__ g, T *__restrict__ dW) {
+  __shared__ int32_t s_key[kMaxEntries + 2], s_pos[kMaxEntries];
+  if ((int32_t)blockIdx.x >= a.blocks) {
+    const int32_t z = (int32_t)blockIdx.x - a.blocks, v = z * kZeroRows + (int32_t)threadIdx.x;
+    bool absent = false;
+    if (v < a.rows) {
+      const int32_t at = lower_bound(a.keys, a.n, v);
+      absent = !(at < a.n && a.keys[at] == v);
+    }
+    zero_rows<T, VEC>(z, absent, a.D, dW);
+    return;
+  }
+  const int per_block = a.G * a.per_group;
+  const int32_t s0 = (int32_t)blockIdx.x * per_block, s1 = (int32_t)min((int64_t)a.n, (int64_t)s0 + per_block);
+  int count = s1 - s0;
+  for (int i = threadIdx.x; i < count; i += 256) {
+    s_key[1 + i] = a.keys[s0 + i];
+    s_pos[i] = a.perm[s0 + i];
+  }
+  if (threadIdx.x == 0) {
+    s_key[0] = s0 > 0 ? a.keys[s0 - 1] : -1;
+    s_key[1 + count] = s1 < a.n ? a.keys[s1] : -1;
+  }
+  __syncthreads();
+  if (s_key[count] >= a.rows) count = lower_bound(s_key + 1, count, a.rows);   // entries that add nothing come last
+  if (count == 0) return;
+  sum_entries<T, VEC, false>(a, g, dW, s_key, s_pos, count, a.per_group, a.pieces + (int64_t)blockIdx.x * 2 * a.D);
+}
+
+// Few ids, one launch: every summing workgroup sorts all of them in LDS, by counting, and takes a share of the
+// sorted entries that begins and ends between rows; the zeroing ones look their rows up in the ids.
+template <typename T, int VEC, typename ID>
+__global__ __launch_bounds__(256) void emb_few_kernel(SumArgs a, const ID *__restrict__ ids, int64_t padding,
+                                                      const T *__restrict__ g, T *__restrict__ dW) {
+  __shared__ alignas(16) uint32_t s_in[kFewIds];
+  __shared__ int32_t s_key[kFewIds + 2], s_pos[kFewIds];
+  const int n = a.n;
+  if ((int32_t)blockIdx.x >= a.blocks) {
+    const int32_t z = (int32_t)blockIdx.x - a.blocks, v = z * kZeroRows + (int32_t)threadIdx.x;
+    s_in[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const int32_t r = key_of(ids[i], a.rows, padding) - z * kZeroRows;
+      if (r >= 0 && r < kZeroRows) s_in[r] = 1;
+    }
+    __syncthreads();
+    zero_rows<T, VEC>(z, v < a.rows && s_in[threadIdx.x] == 0, a.D, dW);
+    return;
+  }
+  // key and position in one word: one comparison orders both
+  uint32_t mine[kFewIds / 256];
+  int before[kFewIds / 256];
+#pragma unroll
+  for (int k = 0; k < kFewIds / 256; ++k) {
+    const int i = k * 256 + threadIdx.x;
+    mine[k] = i < n ? (uint32_t)key_of(ids[i], a.rows, padding) << kFewBits | (uint32_t)i : UINT32_MAX;
+    before[k] = 0;
+    s_in[i] = mine[k];
+  }
+  if (threadIdx.x == 0) s_key[0] = s_key[1 + n] = -1;
+  __syncthreads();
+#pragma unroll 4
+  for (int j = 0; j < n; j += 4) {                       // (words behind the last id are larger than all)
+    const uint4 c = *reinterpret_cast<const uint4 *>(&s_in[j]);
+#pragma unroll
+    for (int k = 0; k < kFewIds / 256; ++k)
+      before[k] += (c.x < mine[k]) + (c.y < mine[k]) + (c.z < mine[k]) + (c.w < mine[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kFewIds / 256; ++k)
+    if (mine[k] != UINT32_MAX) {
+      s_key[1 + before[k]] = (int32_t)(mine[k] >> kFewBits);
+      s_pos[before[k]] = (int32_t)(mine[k] & (kFewIds - 1));
+    }
+  __syncthreads();
+  // the share [lo, hi) of this workgroup, moved up to where a row begins
+  const int32_t *key = s_key + 1;
+  const int valid = lower_bound(key, n, a.rows), share = a.G * a.per_group;
+  int lo = min(valid, (int)blockIdx.x * share), hi = min(valid, lo + share);
+  if (lo > 0 && lo < valid && key[lo] == key[lo - 1]) lo = lower_bound(key, n, key[lo] + 1);
+  if (hi > 0 && hi < valid && key[hi] == key[hi - 1]) hi = lower_bound(key, n, key[hi] + 1);
+  if (lo >= hi) return;
+  sum_entries<T, VEC, true>(a, g, dW, s_key + lo, s_pos + lo, hi - lo, (hi - lo + a.G - 1) / a.G, a.pieces);
 }
 
 // acc += the head pieces of workgroups k0 .. k1, in that order, eight of them in flight
@@ -670,6 +740,14 @@ int launch_sort(const ID *ids, int32_t n, int32_t rows, int64_t padding, const L
   return RK_OK;
 }
 
+template <typename T, int VEC, typename ID>
+int launch_few(const SumArgs &a, const ID *ids, int64_t padding, const void *g, void *dW, hipStream_t st) {
+  const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows);
+  emb_few_kernel<T, VEC, ID><<<(uint32_t)blocks, 256, 0, st>>>(a, ids, padding, (const T *)g, (T *)dW);
+  RK_CHECK_LAUNCH("emb_few_kernel");
+  return RK_OK;
+}
+
 template <typename T, int VEC>
 int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
   const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows);
@@ -716,6 +794,16 @@ int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t i
   hipStream_t st = (hipStream_t)stream;
   int32_t *w = (int32_t *)ws;
   const Layout y = layout_of(n, rows, D, dtype);
+  if (n > 0 && n <= kFewIds && rows < kFewRows - 1) {
+    const SumArgs a = {nullptr, nullptr, (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks, scale, (float *)w};
+#define RK_FEW(T, VEC)                                                          \
+  (id_bytes == 8 ? launch_few<T, VEC>(a, (const int64_t *)ids, padding_idx, grad, d_weight, st) \
+                 : launch_few<T, VEC>(a, (const int32_t *)ids, padding_idx, grad, d_weight, st))
+    if (dtype == RK_F32) return D >= 4 ? RK_FEW(float, 4) : RK_FEW(float, 1);
+    if (dtype == RK_BF16) return D >= 8 ? RK_FEW(__bf16, 8) : RK_FEW(__bf16, 1);
+    return D >= 8 ? RK_FEW(_Float16, 8) : RK_FEW(_Float16, 1);
+#undef RK_FEW
+  }
   if (n > 0) {
     const int rc = id_bytes == 8 ? launch_sort((const int64_t *)ids, (int32_t)n, rows, padding_idx, y, w, st)
                                  : launch_sort((const int32_t *)ids, (int32_t)n, rows, padding_idx, y, w, st);
