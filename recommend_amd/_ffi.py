@@ -232,24 +232,30 @@ def ptr(t):
     return c_void_p(t.ctypes.data)
 
 
-_functions = {}
+TORCH_OPS_PATH = os.path.join(_HERE, "lib", "_torch_ops.so")
+_TORCH_OPS_USES = ("rk_last_error", "rk_embedding_fwd", "rk_embedding_bwd_ws_bytes", "rk_embedding_bwd",
+                   "rk_list_logps_ws_bytes", "rk_list_logps_fwd", "rk_preference_fwd", "rk_list_logps_bwd",
+                   "rk_adamw_ws_bytes", "rk_adamw_step")
+_torch_ops = None
 
 
-def call_on(device, name, *args):
-    """`call` with `device` current (a launch goes to the device its stream belongs to) and that device's
-    current stream as the last argument."""
-    import torch
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = getattr(load(), name)
-    index = device.index
-    if torch.cuda.current_device() == index:
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if code != RK_OK:
-        check(code)
+def torch_ops():
+    """The Python module of the operators whose host side is C++ (csrc/torch_ops.cpp), on this process's library."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (the module's symbols come from torch's libraries)
+        if not os.path.exists(TORCH_OPS_PATH):
+            raise RkError(RK_ERR_NODEV, f"{TORCH_OPS_PATH} is missing: run `python -m recommend_amd.build` "
+                          "(or __graft_entry__.build()) first; there is no Python fallback")
+        spec = importlib.util.spec_from_file_location("_torch_ops", TORCH_OPS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        lib = load()
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _TORCH_OPS_USES}, RkError)
+        _torch_ops = module
+    return _torch_ops
 
 
 def stream_ptr(device=None):
@@ -257,7 +263,7 @@ def stream_ptr(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-__all__ = ["load", "call", "call_on", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "AdamwTensor", "AdamwGroup",
+__all__ = ["load", "call", "torch_ops", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "AdamwTensor", "AdamwGroup",
            "RkError", "SIGNATURES",
            "LIB_PATH", "device_count", "require_device", "last_error",
            "c_int32", "c_int64", "c_float", "c_double", "c_uint32", "c_size_t"]

@@ -2,6 +2,7 @@
 
 The library is the C-ABI declared in include/recommend_amd.h; it is built here
 on a CPU-only host (hipcc cross-compiles) and travels to the GPU box as a file.
+Beside it _torch_ops.so, a Python module of host code (g++).
 """
 import os
 import subprocess
@@ -24,10 +25,29 @@ FLAGS = [
 ]
 
 
+# the operators' torch side (argument checks, buffers, autograd nodes): host code against torch's own headers
+TORCH_OPS = "torch_ops.cpp"
+TORCH_OPS_PATH = os.path.join(LIB_DIR, "_torch_ops.so")
+
+
+def torch_ops_command(out):
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__=1",
+            "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+            "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(rocm, "include"),
+            os.path.join(CSRC, TORCH_OPS), "-o", out, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_hip", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
 def needs_build():
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(TORCH_OPS_PATH):
         return True
-    t = os.path.getmtime(LIB_PATH)
+    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TORCH_OPS_PATH))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(HERE, "..", "include", "recommend_amd.h"))
     deps.append(os.path.abspath(__file__))
@@ -49,9 +69,13 @@ def build(force=False, verbose=True):
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd)))
         objs.append(obj)
+    cmd = torch_ops_command(TORCH_OPS_PATH)
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    procs.append((TORCH_OPS, subprocess.Popen(cmd)))
     for src, p in procs:
         if p.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {src}")
+            raise RuntimeError(f"the compiler failed on {src}")
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -35,8 +35,8 @@ constexpr int kFewBits = 9, kFewIds = 1 << kFewBits;   // ids that every summing
 constexpr int32_t kFewRows = 1 << (32 - kFewBits);      // (key and position have to fit a word)
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
 constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
-constexpr int kPerGroup = 16;         // sorted entries of a lane group
-constexpr int kJoins = 16;            // workgroup borders that one workgroup of the closing launch looks at
+constexpr int kPerGroup = 32;         // sorted entries of a lane group
+constexpr int kJoins = 4;             // workgroup borders that one workgroup of the closing launch looks at
 constexpr int64_t kStreamBytes = 64 << 20;   // looked-up rows from this size on are stored past the caches
 constexpr int kLongRun = 8;          // workgroup pieces of a row above which a whole workgroup joins them
 

@@ -137,9 +137,6 @@ def sgrec_loss(result, batch, reg_weight=0.0):
     return loss + reg_weight * reg_loss
 
 
-_PREFERENCE_KINDS = {"sigmoid": ops.PREF_SIGMOID, "hinge": ops.PREF_HINGE, "squared": ops.PREF_SQUARED}
-
-
 def list_logps(scores, items, ignore_index=-100, average=False):
     """Log-probabilities of item lists under catalogue scores (see ops.list_logps): what a frozen
     reference model says goes into preference_loss as `ref_logps`."""
@@ -158,27 +155,9 @@ def preference_loss(scores, items, ref_logps, beta=0.1, label_smoothing=0.0, kin
       "sigmoid"  -(1 - label_smoothing) logsigmoid(beta d) - label_smoothing logsigmoid(-beta d)
       "hinge"    max(0, 1 - beta d)
       "squared"  (d - 1 / (2 beta))^2
-    Returns (mean over the pairs, logps [2P]); both are differentiable with respect to scores, so a term
-    on the preferred lists' own log-probabilities can be added."""
-    if kind not in _PREFERENCE_KINDS:
-        raise ValueError(f"preference_loss: kind is one of {sorted(_PREFERENCE_KINDS)}, not {kind!r}")
-    if not beta > 0:
-        raise ValueError("preference_loss: beta must be positive")
-    if not 0 <= label_smoothing <= 1:
-        raise ValueError("preference_loss: label_smoothing outside [0, 1]")
-    if label_smoothing and kind != "sigmoid":
-        raise ValueError("preference_loss: label smoothing is part of the sigmoid form only")
-    S = scores.shape[0]
-    if S < 2 or S % 2:
-        raise ValueError(f"preference_loss: pairs of lists are needed, got {S} lists")
-    if tuple(ref_logps.shape) != (S,):
-        raise ValueError(f"preference_loss: one reference log-probability per list, got {tuple(ref_logps.shape)} for {S}")
-    items = ops._list_args(scores, items, "preference_loss")
-    ops._same_device(scores, ref_logps)
-    logps, loss = ops._ListLogps.apply(scores, items, ops._f32c(ref_logps.detach()),
-                                       (int(ignore_index), int(bool(average)), float(beta), float(label_smoothing),
-                                        _PREFERENCE_KINDS[kind]))
-    return loss, logps
+    Returns (mean over the pairs, logps [2P]); both are differentiable (once) with respect to scores, so a
+    term on the preferred lists' own log-probabilities can be added."""
+    return _ffi.torch_ops().preference_loss(scores, items, ref_logps, beta, label_smoothing, kind, ignore_index, average)
 
 
 __all__ = ["bpr_loss", "gather_dot_bpr_loss", "mmgcn_loss", "compute_info_bpr_loss", "sgrec_loss", "list_logps",

@@ -407,87 +407,8 @@ def bpr_gather_dot_sampled(U, I, users, pos, neg_rank, pos_ptr, pos_items, mask=
 
 # --------------------------------------------------------------------------
 # embedding lookup with scaling; log-probabilities of item lists
+# (checks, buffers and autograd nodes: csrc/torch_ops.cpp)
 # --------------------------------------------------------------------------
-_MAX_INT = 2 ** 31 - 2 ** 24     # sizes are int32 at the C boundary
-_ELEM = {torch.float32: _ffi.F32, torch.bfloat16: _ffi.BF16, torch.float16: _ffi.F16}
-
-
-def _elem(t, what):
-    code = _ELEM.get(t.dtype)
-    if code is None:
-        raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, f"{what}: float32, bfloat16 or float16, not {t.dtype}")
-    return code
-
-
-def _scratch(nbytes, device):
-    return torch.empty((nbytes + 7) // 8, dtype=torch.float64, device=device)
-
-
-def _same_device(*tensors):
-    """All of them on one HIP device."""
-    _need_cuda(*tensors)
-    dev = tensors[0].device
-    for t in tensors[1:]:
-        if t.device != dev:
-            raise ValueError(f"tensors on several devices: {dev} and {t.device}")
-
-
-def _once(backward):
-    """A backward pass without a derivative of its own, as torch's once_differentiable, whose bookkeeping is
-    entered only where a graph of the gradient is asked for."""
-    slow = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return run
-
-
-class _NoSecondDerivative(torch.autograd.Function):
-    """The identity on a gradient that depends on saved inputs (once_differentiable takes it for a constant where
-    the upstream gradient is one): differentiating it raises."""
-
-    @staticmethod
-    def forward(ctx, x):
-        return x.view_as(x)
-
-    @staticmethod
-    def backward(ctx, g):
-        raise RuntimeError("the list operators are differentiable once: they have no second derivative")
-
-
-class _EmbeddingLookup(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, ids, args):       # args: (scale, padding_idx)
-        ctx.save_for_backward(ids)
-        ctx.args, ctx.shape = args, weight.shape
-        return _embedding_fwd(weight, ids, args[0])
-
-    @staticmethod
-    @_once
-    def backward(ctx, g):
-        ids, = ctx.saved_tensors
-        (rows, D), (scale, padding_idx) = ctx.shape, ctx.args
-        g = g.contiguous()
-        dev, kind, n = g.device, _ELEM[g.dtype], ids.numel()
-        dw = torch.empty((rows, D), dtype=g.dtype, device=dev)
-        ws = _scratch(_ffi.load().rk_embedding_bwd_ws_bytes(n, rows, D, kind), dev)
-        _ffi.call_on(dev, "rk_embedding_bwd", g.data_ptr(), kind, ids.data_ptr(), ids.element_size(), n, rows, D, scale,
-                     padding_idx, dw.data_ptr(), ws.data_ptr(), ws.numel() * 8)
-        return dw, None, None
-
-
-def _embedding_fwd(w, ids, scale):
-    rows, D = w.shape
-    ld, step = w.stride()
-    if step != 1 or ld < D:
-        w, ld = w.contiguous(), D
-    dev = w.device
-    out = torch.empty((*ids.shape, D), dtype=w.dtype, device=dev)
-    _ffi.call_on(dev, "rk_embedding_fwd", w.data_ptr(), ld, rows, D, _ELEM[w.dtype], ids.data_ptr(), ids.element_size(),
-                 ids.numel(), scale, out.data_ptr())
-    return out
-
-
 def embedding_lookup(weight, ids, scale=1.0, padding_idx=None):
     """scale * weight[ids] with a deterministic gradient (rk_embedding_fwd / rk_embedding_bwd).
 
@@ -495,120 +416,9 @@ def embedding_lookup(weight, ids, scale=1.0, padding_idx=None):
     of the table's type (the product is taken in fp32 and rounded once).  The gradient of `weight` is
     dense; contributions of equal ids are added in fp32 in the order of their positions, the same bits
     on every run, and positions whose id is `padding_idx` (negative values count from the end, as in
-    torch.nn.Embedding) add nothing.  An id outside the table gives a row of NaN and no gradient."""
-    if weight.dim() != 2 or weight.shape[1] < 1:
-        raise ValueError(f"embedding_lookup: the table is [rows, D], got {tuple(weight.shape)}")
-    if weight.dtype not in _ELEM:
-        _elem(weight, "embedding_lookup")
-    if max(weight.shape) >= _MAX_INT:
-        raise ValueError(f"embedding_lookup: a table of {tuple(weight.shape)} has more than 2^31 rows or columns")
-    if ids.dtype != torch.int64 and ids.dtype != torch.int32:
-        raise ValueError(f"embedding_lookup: ids are int32 or int64, not {ids.dtype}")
-    if padding_idx is None:
-        padding_idx = -1
-    else:
-        rows = weight.shape[0]
-        if not -rows <= padding_idx < rows:
-            raise ValueError(f"embedding_lookup: padding_idx {padding_idx} outside the table of {rows} rows")
-        padding_idx = int(padding_idx) % rows
-    _same_device(weight, ids)
-    ids = ids.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
-        return _EmbeddingLookup.apply(weight, ids, (float(scale), padding_idx))
-    return _embedding_fwd(weight.detach(), ids, float(scale))
-
-
-PREF_SIGMOID, PREF_HINGE, PREF_SQUARED = 0, 1, 2   # RK_PREF_* of the header
-
-
-def _list_args(scores, items, what):
-    """Checks a list operator's scores and items; returns the items as contiguous int64."""
-    if scores.dtype not in _ELEM:
-        _elem(scores, what)
-    if items.dtype != torch.int64 and items.dtype != torch.int32:
-        raise ValueError(f"{what}: items are int32 or int64, not {items.dtype}")
-    if scores.dim() not in (2, 3) or scores.shape[:-1] != items.shape:
-        raise ValueError(f"{what}: scores [lists, places, catalogue] and items [lists, places] (or without places), "
-                         f"got {tuple(scores.shape)} and {tuple(items.shape)}")
-    if 0 in scores.shape[1:]:
-        raise ValueError(f"{what}: no places or no catalogue in {tuple(scores.shape)}")
-    if max(scores.shape) >= _MAX_INT:
-        raise ValueError(f"{what}: more than 2^31 lists, places or items in {tuple(scores.shape)}")
-    _same_device(scores, items)
-    return items.to(torch.int64).contiguous()
-
-
-def _list_geometry(scores, items):
-    """Arguments that describe scores and items to the rk_list_logps_* / rk_preference_* calls."""
-    if scores.dim() == 3:
-        (S, T, V), (ss, st, _) = scores.shape, scores.stride()
-    else:
-        (S, V), (ss, _), T, st = scores.shape, scores.stride(), 1, 0
-    return scores.data_ptr(), _ELEM[scores.dtype], S, T, V, ss, st, items.data_ptr(), T
-
-
-class _ListLogps(torch.autograd.Function):
-    """logps [S]; with ref_logps also the preference loss of the pairs (s, S/2 + s)."""
-
-    @staticmethod
-    def forward(ctx, scores, items, ref, args):      # args: (ignore_index, average, beta, label_smoothing, kind)
-        if scores.stride(-1) != 1 and scores.shape[-1] != 1:
-            scores = scores.contiguous()
-        geo = _list_geometry(scores, items)
-        dev, S, rows = scores.device, geo[2], items.numel()
-        ctx.set_materialize_grads(False)
-        ignore_index, average, beta, smoothing, kind = args
-        ctx.args = (ignore_index, average, ref is not None)
-        logps = torch.empty(S, dtype=torch.float32, device=dev)
-        if S == 0:
-            ctx.save_for_backward(scores, items, logps)
-            return (logps,)
-        # (max, log sum) of every row, used places and slopes of every list: kept for the backward pass;
-        # behind them the call's workspace
-        n_keep = 2 * rows + 2 * S
-        n_keep += n_keep % 2
-        ws_bytes = _ffi.load().rk_list_logps_ws_bytes(S, geo[3], geo[4])
-        keep = torch.empty(n_keep + (ws_bytes + 3) // 4, dtype=torch.float32, device=dev)
-        ctx.save_for_backward(scores, items, keep)
-        stat = keep.data_ptr()
-        used, ws = stat + 8 * rows, stat + 4 * n_keep
-        if ref is None:
-            _ffi.call_on(dev, "rk_list_logps_fwd", *geo, ignore_index, average, stat, logps.data_ptr(), used, ws, ws_bytes)
-            return (logps,)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        _ffi.call_on(dev, "rk_preference_fwd", *geo, ignore_index, average, ref.data_ptr(), beta, smoothing, kind, stat,
-                     logps.data_ptr(), used, used + 4 * S, loss.data_ptr(), ws, ws_bytes)
-        return logps, loss
-
-    @staticmethod
-    def backward(ctx, g_logps, g_loss=None):
-        if not torch.is_grad_enabled():
-            return _ListLogps._gradients(ctx, g_logps, g_loss)
-        with torch.no_grad():
-            dx = _ListLogps._gradients(ctx, g_logps, g_loss)[0]
-        return (None if dx is None else _NoSecondDerivative.apply(dx.requires_grad_(True))), None, None, None
-
-    @staticmethod
-    def _gradients(ctx, g_logps, g_loss):
-        scores, items, keep = ctx.saved_tensors
-        ignore_index, average, pairs = ctx.args
-        if g_logps is None and g_loss is None:
-            return (None,) * 4
-        dev = scores.device
-        dx = torch.empty(scores.shape, dtype=scores.dtype, device=dev)
-        geo = _list_geometry(scores, items)
-        S = geo[2]
-        if S:
-            if g_logps is not None:
-                g_logps = _f32c(g_logps)
-            if g_loss is not None:
-                g_loss = _f32c(g_loss)
-            stat = keep.data_ptr()
-            used = stat + 8 * items.numel()
-            _ffi.call_on(dev, "rk_list_logps_bwd", *geo, ignore_index, average, stat, used,
-                         None if g_loss is None else g_loss.data_ptr(), used + 4 * S if pairs else None,
-                         None if g_logps is None else g_logps.data_ptr(), dx.data_ptr())
-        return dx, None, None, None
+    torch.nn.Embedding) add nothing.  An id outside the table gives a row of NaN and no gradient.
+    Differentiable once."""
+    return _ffi.torch_ops().embedding_lookup(weight, ids, scale, padding_idx)
 
 
 def list_logps(scores, items, ignore_index=-100, average=False):
@@ -618,9 +428,8 @@ def list_logps(scores, items, ignore_index=-100, average=False):
     scores: [S, T, V] (or [S, V]) fp32, bfloat16 or fp16, rows of V contiguous, any strides between
     them; items: [S, T] (or [S]) int32 or int64, `ignore_index` where a place is not in use (its scores are
     not read and get a gradient of zero).  A list without places in use has 0; an item outside the
-    catalogue makes its list NaN.  Returns fp32 [S], differentiable with respect to scores."""
-    items = _list_args(scores, items, "list_logps")
-    return _ListLogps.apply(scores, items, None, (int(ignore_index), int(bool(average)), 0.0, 0.0, 0))[0]
+    catalogue makes its list NaN.  Returns fp32 [S], differentiable (once) with respect to scores."""
+    return _ffi.torch_ops().list_logps(scores, items, ignore_index, average)
 
 
 # --------------------------------------------------------------------------

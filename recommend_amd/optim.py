@@ -16,7 +16,6 @@ Several GPUs: parameters listed in `sharded_params` are row shards (every rank h
 their squared gradient norms are summed over the ranks of `group` by one all-reduce of one float
 between the two launches (rk_adam_sqnorm_f32 / rk_adam_update_f32).  All other parameters are
 taken to be replicated with gradients already summed over the ranks."""
-import numpy as np
 import torch
 
 from . import _ffi
@@ -167,7 +166,6 @@ class FusedClipAdam(torch.optim.Optimizer):
             self._lr_host = lr
 
 
-_DTYPES = {torch.float32: _ffi.F32, torch.bfloat16: _ffi.BF16, torch.float16: _ffi.F16}
 _FULL = 448.0       # largest finite e4m3 value
 _TINY = 1e-30       # block maxima below this count as this
 _STATE32 = ("exp_avg", "exp_avg_sq")
@@ -265,6 +263,7 @@ class FusedAdamW(torch.optim.Optimizer):
         self.step_count = torch.full((1,), self._restored_step, dtype=torch.int64, device=dev)
         self.lr_dev = torch.zeros(_ffi.ADAMW_MAX_GROUPS, dtype=torch.float32, device=dev)
         self.grad_norm = torch.zeros(1, dtype=torch.float32, device=dev)
+        self._ws = torch.empty(0, dtype=torch.float64, device=dev)
 
     def _refuse(self, p, g):
         if not p.is_cuda:
@@ -274,56 +273,30 @@ class FusedAdamW(torch.optim.Optimizer):
         raise _ffi.RkError(_ffi.RK_ERR_UNSUPPORTED, "FusedAdamW: contiguous fp32, bfloat16 or fp16 parameters on a HIP "
                            "device with dense gradients of their type or fp32 only")
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        rows, dev, state, strided = [], self._dev, self.state, torch.strided
-        for k, group in enumerate(self.param_groups):
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                n = p.numel()
-                if n == 0:
-                    continue
-                if dev is None:
-                    if not p.is_cuda:
-                        self._refuse(p, g)
-                    self._init_device(p.device)
-                    dev = self._dev
-                pd, gd = _DTYPES.get(p.dtype), _DTYPES.get(g.dtype)
-                if not (pd is not None and (gd == pd or gd == 0) and g.layout is strided and p.is_contiguous()
-                        and g.is_contiguous() and p.device == dev and g.device == dev):
-                    self._refuse(p, g)
-                st = state[p]
-                if "exp_avg8" not in st and "exp_avg" not in st:
-                    st = self._state_for(p)
-                if "exp_avg8" in st:
-                    rows.append((p.data_ptr(), g.data_ptr(), st["exp_avg8"].data_ptr(), st["exp_avg_sq8"].data_ptr(),
-                                 st["exp_avg8_scale"].data_ptr(), st["exp_avg_sq8_scale"].data_ptr(), n, pd | gd << 32, k))
-                else:
-                    rows.append((p.data_ptr(), g.data_ptr(), st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr(), 0, 0, n,
-                                 pd | gd << 32, k))
-        if not rows:
-            return loss
-        n = len(rows)
-        table = np.array(rows, np.int64)             # n rows of rk_adamw_tensor (its int32 pairs as one int64 each)
-        groups = (_ffi.AdamwGroup * len(self.param_groups))()
-        for dst, group in zip(groups, self.param_groups):
-            (dst.beta1, dst.beta2), dst.eps, dst.weight_decay = group["betas"], group["eps"], group["weight_decay"]
+        if self._dev is None:
+            first = next((p for g in self.param_groups for p in g["params"] if p.grad is not None and p.numel()), None)
+            if first is None:
+                return loss
+            if not first.is_cuda:
+                self._refuse(first, first.grad)
+            self._init_device(first.device)
         self.sync_lr()
-        need = _ffi.load().rk_adamw_ws_bytes(n)
-        if self._ws is None or self._ws.numel() * 8 < need:
+        need = self._launch()
+        if need:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
-            self._ws = torch.empty(need // 8, dtype=torch.float64, device=dev)
-        _ffi.call_on(dev, "rk_adamw_step", table.ctypes.data, n, groups, len(groups), self.step_count.data_ptr(),
-                     self.lr_dev.data_ptr(), float(self.max_grad_norm or 0.0), self.grad_norm.data_ptr(),
-                     self._ws.data_ptr(), self._ws.numel() * 8)
+            self._ws = torch.empty(need // 8, dtype=torch.float64, device=self._dev)
+            self._launch()
         return loss
+
+    def _launch(self):
+        return _ffi.torch_ops().adamw_step(self.param_groups, self.state, self._state_for, self._refuse, self.step_count,
+                                           self.lr_dev, self.max_grad_norm or 0.0, self.grad_norm, self._ws)
 
     def sync_lr(self):
         """Push learning rates changed by a scheduler to device memory (step() does it; call it for a step that

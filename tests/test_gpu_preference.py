@@ -11,7 +11,6 @@ import pytest
 import torch
 
 from recommend_amd.loss import list_logps, preference_loss
-from recommend_amd import ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -276,4 +275,3 @@ def test_recorded_in_a_graph_and_replayed_beside_eager_work():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(recorded, eager))
-    assert ops.PREF_SIGMOID == 0
