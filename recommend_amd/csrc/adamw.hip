@@ -30,11 +30,16 @@ namespace {
 constexpr int kMaxTensors = 48;
 constexpr int kMaxGroups = RK_ADAMW_MAX_GROUPS;
 constexpr int kChunk = 2048;         // elements of a workgroup of the update
-constexpr int kNormChunk = 8192;     // elements that a workgroup of the squared-norm launch takes at a time
+constexpr int kNormVectors = 8;      // 16-byte vectors of a lane that the squared-norm launch has in flight
 constexpr int kNormBlocks = 2048;    // its workgroups
 constexpr int kBlock = RK_ADAMW_BLOCK;
 constexpr float kFull = 448.0f;      // largest finite e4m3 value
 constexpr float kTiny = 1e-30f;      // block maxima below this count as this
+
+// elements that a workgroup of the squared-norm launch takes at a time
+__host__ __device__ __forceinline__ int norm_chunk(int grad_dtype) {
+  return kNormVectors * 256 * (grad_dtype == RK_F32 ? 4 : 8);
+}
 
 struct Tensor {
   void *param;
@@ -116,7 +121,7 @@ __global__ __launch_bounds__(256) void adamw_begin_kernel(GroupsIn gr, const flo
 // sum of squares of g[lo .. hi) (a chunk), in 64 bits, all vectors of a lane in flight
 template <typename T>
 __device__ __forceinline__ double square_sum(const T *__restrict__ g, int64_t lo, int64_t hi) {
-  constexpr int VEC = rk::Elem<T>::kVec, U = kNormChunk / (256 * VEC);
+  constexpr int VEC = rk::Elem<T>::kVec, U = kNormVectors;
   double s[2] = {0.0, 0.0};
   int64_t i = lo + (int64_t)threadIdx.x * VEC;
   for (; i + (U - 1) * 256 * VEC + VEC <= hi; i += U * 256 * VEC) {
@@ -157,8 +162,8 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(Args a, double *__restr
   for (int32_t c = blockIdx.x, i = 0; c < chunks; c += (int32_t)gridDim.x) {
     while (a.chunk_start[i + 1] <= c) ++i;
     const Tensor &t = a.t[i];
-    const int64_t lo = (int64_t)(c - a.chunk_start[i]) * kNormChunk, hi = min(t.n, lo + kNormChunk);
     const int gd = t.kind >> 2;
+    const int64_t lo = (int64_t)(c - a.chunk_start[i]) * norm_chunk(gd), hi = min(t.n, lo + norm_chunk(gd));
     if (gd == RK_F32)
       s += square_sum((const float *)t.grad, lo, hi);
     else if (gd == RK_BF16)
@@ -442,7 +447,7 @@ int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors, const 
         a.t[i] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.n,
                   t.param_dtype | t.grad_dtype << 2, t.group};
         a.chunk_start[i] = c;
-        c += (int32_t)rk::ceil_div(t.n, pass == 0 ? kNormChunk : kChunk);
+        c += (int32_t)rk::ceil_div(t.n, pass == 0 ? norm_chunk(t.grad_dtype) : kChunk);
       }
       a.chunk_start[a.n] = c;
       if (pass == 0) {

@@ -184,25 +184,47 @@ __device__ __forceinline__ float pair_term(float d, float beta, float eps, int k
   return term;
 }
 
-// One workgroup: the pairs' terms, their slopes and the mean, added in a fixed order.  ROWS: it also forms the
-// lists' log-probabilities, from up to kFewRows rows, a thread for each (one launch instead of two).
-template <bool ROWS>
+// One workgroup: the pairs' terms, their slopes and the mean, added in a fixed order.  K > 0: it also forms the
+// lists' log-probabilities, from up to K rows for each thread (one launch instead of two).
+template <int K>
 __global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float2 *__restrict__ part,
                                                              const float *__restrict__ score, float2 *__restrict__ stat,
                                                              const float *__restrict__ ref, int average, float beta,
                                                              float eps, int kind, float *__restrict__ logps,
                                                              int32_t *__restrict__ used, float *__restrict__ slope_out,
                                                              float *__restrict__ loss) {
-  __shared__ float s_row[ROWS ? kFewRows : 1], s_logp[ROWS ? kFewRows : 1];
+  constexpr bool ROWS = K > 0;
+  __shared__ float s_row[ROWS ? K * kPairThreads : 1], s_logp[ROWS ? K * kPairThreads : 1];
   __shared__ double s_sum[kPairThreads / rk::kWave];
   const int32_t P = a.S / 2;
   if constexpr (ROWS) {
     const int32_t rows = a.S * a.T;
-    for (int32_t row = threadIdx.x; row < rows; row += kPairThreads) {
-      const int32_t s = row / a.T, t = row - s * a.T;
-      const bool in = a.items[s * a.ld_items + t] != a.ignore;
+    bool in[K];                                            // (the loads of a thread's rows are in flight together)
+    float m[K], q[K], sc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int32_t row = min(k * kPairThreads + (int32_t)threadIdx.x, rows - 1), s = row / a.T, t = row - s * a.T;
+      in[k] = k * kPairThreads + (int32_t)threadIdx.x < rows && a.items[s * a.ld_items + t] != a.ignore;
+      sc[k] = score[row];                                  // (not written for a place that is not in use, and not used)
+      m[k] = -__FLT_MAX__;
+      q[k] = 0.0f;
+    }
+    for (int p = 0; p < a.parts; ++p) {
+      float2 o[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        o[k] = part[(int64_t)min(k * kPairThreads + (int32_t)threadIdx.x, rows - 1) * a.parts + p];
+#pragma unroll
+      for (int k = 0; k < K; ++k) merge(m[k], q[k], o[k].x, o[k].y);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int32_t row = k * kPairThreads + (int32_t)threadIdx.x;
+      if (row >= rows) break;
+      const float lq = logf(q[k]);
+      if (in[k]) stat[row] = make_float2(m[k], lq);
       // a place that is not in use is marked by the one value that no log-probability has
-      s_row[row] = in ? row_logp(a, row, part, score, stat) : __builtin_inff();
+      s_row[row] = in[k] ? (sc[k] - m[k]) - lq : __builtin_inff();
     }
     __syncthreads();
     // 16 lanes for every list
@@ -395,14 +417,19 @@ int run_pairs(const Rows &a, const void *x, const float *ref, int average, float
   const Ws w = ws_of(a);
   if (int rc = launch_rows_fwd<T>(a, x, ws, w, st)) return rc;
   const float2 *part = (const float2 *)(ws + w.part);
-  if ((int64_t)a.S * a.T <= kFewRows) {
-    pairs_kernel<true><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind, logps,
-                                                  used, slope, loss);
+  const int64_t rows = (int64_t)a.S * a.T;
+#define RK_PAIRS(K)                                                                                                    \
+  pairs_kernel<K><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind, logps, \
+                                              used, slope, loss)
+  if (rows <= kPairThreads) {
+    RK_PAIRS(1);
+  } else if (rows <= kFewRows) {
+    RK_PAIRS(kFewRows / kPairThreads);
   } else {
     if (int rc = launch_lists(a, average, stat, logps, used, ws, w, st)) return rc;
-    pairs_kernel<false><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind,
-                                                   logps, used, slope, loss);
+    RK_PAIRS(0);
   }
+#undef RK_PAIRS
   RK_CHECK_LAUNCH("pairs_kernel");
   return RK_OK;
 }
