@@ -9,12 +9,12 @@ from . import _ffi
 from ._ffi import RkError
 from .graph_constructor import GraphConstructor, DeviceGraph
 from .evaluator import Verifier, Tester, RankingEvaluator
-from .loss import bpr_loss, gather_dot_bpr_loss
+from .loss import bpr_loss, gather_dot_bpr_loss, list_logps, preference_loss
 from .sampler import NegativeSampler, TrainBatchLoader, build_user_csr
 from .model import TESTModel, ModelFactory
 from .data import InteractionTable, InteractionSplit, mask_index
 
 __all__ = ["GraphConstructor", "DeviceGraph", "Verifier", "Tester", "RankingEvaluator",
-           "bpr_loss", "gather_dot_bpr_loss", "NegativeSampler", "TrainBatchLoader",
+           "bpr_loss", "gather_dot_bpr_loss", "list_logps", "preference_loss", "NegativeSampler", "TrainBatchLoader",
            "build_user_csr", "TESTModel", "ModelFactory", "RkError", "InteractionTable",
            "InteractionSplit", "mask_index"]

@@ -1,4 +1,6 @@
-"""Adam with global-norm gradient clipping on the library's two-launch kernel pair
+"""The optimizers on the library's kernels: FusedClipAdam, and FusedAdamW (rk_adamw_step; described there).
+
+FusedClipAdam is Adam with global-norm gradient clipping on the two-launch kernel pair
 (rk_adam_clip_step_f32): the optimizer half of train/graph_trainer.py:151-156,
 `clip_grad_norm_(model.parameters(), max_norm); optimizer.step()`, for fp32 parameters.
 
