@@ -412,8 +412,9 @@ int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors, const 
     gr.g[g] = {s.beta1, s.beta2, s.weight_decay};
     hy.g[g] = {(float)s.beta1, (float)(1.0 - s.beta1), (float)s.beta2, (float)(1.0 - s.beta2), (float)s.eps};
   }
-  int64_t chunks = 0;
+  int64_t chunks = 0;                 // of the update's current launch
   for (int i = 0; i < n_tensors; ++i) {
+    if (i % kMaxTensors == 0) chunks = 0;
     const rk_adamw_tensor &t = tensors_host[i];
     RK_CHECK_ARG(t.n > 0 && t.param && t.grad && t.exp_avg && t.exp_avg_sq, "tensor %d: null pointer or empty", i);
     RK_CHECK_ARG(!t.exp_avg_scale == !t.exp_avg_sq_scale, "tensor %d: one of the two scales is missing", i);
@@ -425,8 +426,8 @@ int rk_adamw_step(const rk_adamw_tensor *tensors_host, int32_t n_tensors, const 
     RK_CHECK_ARG(!t.exp_avg_scale || (((uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq) & 3) == 0,
                  "tensor %d: 8-bit moments must be 4-byte aligned", i);
     chunks += rk::ceil_div(t.n, kChunk);
+    RK_CHECK_ARG(chunks < rk::kMaxBlocks256, "too many elements in one launch's tensors");
   }
-  RK_CHECK_ARG(chunks < INT32_MAX, "too many elements");
   hipStream_t st = (hipStream_t)stream;
   Factors *f = (Factors *)ws;
   double *partial = (double *)((char *)ws + kPartialAt);

@@ -99,6 +99,7 @@ struct Pack {
   }
 };
 
-static inline int elem_size(int32_t dtype) { return dtype == RK_F32 ? 4 : 2; }
+// workgroups of 256 threads in one dimension of a grid, which is counted in threads, in 32 bits
+constexpr int64_t kMaxBlocks256 = (1ll << 32) / 256 - 1;
 
 }  // namespace rk

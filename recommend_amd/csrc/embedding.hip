@@ -96,7 +96,7 @@ template <typename ID>
 __global__ __launch_bounds__(256) void emb_rank_sort_kernel(const ID *__restrict__ ids, int32_t n, int32_t rows,
                                                             int64_t padding, int32_t *__restrict__ keys,
                                                             int32_t *__restrict__ perm) {
-  __shared__ int32_t s_key[kRankSortMax];
+  __shared__ alignas(16) int32_t s_key[kRankSortMax];
   const int32_t room = (n + 3) / 4 * 4;
   for (int j = threadIdx.x; j < room; j += 256) s_key[j] = j < n ? key_of(ids[j], rows, padding) : INT32_MAX;
   __syncthreads();
@@ -690,7 +690,7 @@ template <typename T, int VEC, typename ID, int ROWS, bool ONCE>
 int launch_fwd_as(const void *W, int64_t ldw, int32_t rows, int32_t D, const void *ids, int64_t n, float scale, void *out,
                   int L, hipStream_t st) {
   const int64_t blocks = rk::ceil_div(n, (int64_t)(256 / L) * ROWS);
-  RK_CHECK_ARG(blocks < INT32_MAX, "too many ids");
+  RK_CHECK_ARG(blocks < rk::kMaxBlocks256, "too many ids for one call");
   emb_fwd_kernel<T, VEC, ID, ROWS, ONCE><<<(uint32_t)blocks, 256, 0, st>>>((const T *)W, ldw, rows, D, (const ID *)ids, n,
                                                                          scale, L, (T *)out);
   RK_CHECK_LAUNCH("emb_fwd_kernel");
@@ -751,6 +751,7 @@ int launch_few(const SumArgs &a, const ID *ids, int64_t padding, const void *g, 
 template <typename T, int VEC>
 int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
   const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows);
+  RK_CHECK_ARG(blocks < rk::kMaxBlocks256, "too many ids for one call");
   emb_sum_kernel<T, VEC><<<(uint32_t)blocks, 256, 0, st>>>(a, (const T *)g, (T *)dW);
   RK_CHECK_LAUNCH("emb_sum_kernel");
   if (a.blocks > 1) {
