@@ -23,6 +23,8 @@ constexpr int kWaves = kThreads / rk::kWave;
 constexpr int kPairThreads = 1024;
 constexpr int kFewRows = 4096;       // rows that one workgroup joins
 
+// A row's part is read by a workgroup, or by a wavefront (four parts in a workgroup): a row of 1000 scores
+// keeps 125 of 256 threads busy once.
 struct Rows {
   int64_t stride_s, stride_t;   // of the scores, in elements
   int32_t S, T, V;              // lists, places, catalogue
@@ -30,7 +32,15 @@ struct Rows {
   const int64_t *items;         // [S, T]
   int64_t ld_items;
   int64_t ignore;
+  uint32_t units;               // S * T * parts, below 2^31
 };
+
+// which (row, part) a thread works on: the grid has two dimensions because one ends at 2^32 threads
+template <int TPR>
+__device__ __forceinline__ uint32_t unit_index() {   // (units < 2^31; the same for a wavefront, kept in scalar registers)
+  const uint32_t block = blockIdx.y * gridDim.x + blockIdx.x;
+  return TPR == kThreads ? block : __builtin_amdgcn_readfirstlane(block * (kThreads / TPR) + threadIdx.x / TPR);
+}
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
@@ -44,18 +54,21 @@ __device__ __forceinline__ void merge(float &m, float &s, float om, float os) {
 
 // One part of one row: its (max, sum) and, if the row's item lies in it, the item's score.  The next step's
 // vectors are on their way while a step's exponentials are computed.
-template <typename T>
+template <typename T, int TPR>   // TPR: threads of a part, 256 or 64
 __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__restrict__ x, float2 *__restrict__ part,
                                                             float *__restrict__ score) {
-  constexpr int VEC = rk::Elem<T>::kVec, U = 4, kStep = U * kThreads * VEC;
+  constexpr int VEC = rk::Elem<T>::kVec, U = 4, kStep = U * TPR * VEC;
   __shared__ float s_m[kWaves], s_s[kWaves];
-  const int64_t row = blockIdx.x / a.parts;
-  const int32_t p = (int32_t)(blockIdx.x - row * a.parts), s = (int32_t)(row / a.T), t = (int32_t)(row - (int64_t)s * a.T);
+  const uint32_t unit = unit_index<TPR>();
+  if (unit >= a.units) return;
+  const int lane = TPR == kThreads ? threadIdx.x : threadIdx.x % TPR;
+  const uint32_t row = unit / (uint32_t)a.parts;
+  const int32_t p = (int32_t)(unit - row * a.parts), s = (int32_t)(row / (uint32_t)a.T), t = (int32_t)(row - (uint32_t)s * a.T);
   const int64_t y = a.items[s * a.ld_items + t];
   if (y == a.ignore) return;
   const int32_t lo = p * a.part_len, hi = min(a.V, lo + a.part_len);
   const T *r = x + s * a.stride_s + t * a.stride_t;
-  if (threadIdx.x == 0) {
+  if (lane == 0) {
     if (y >= lo && y < hi)
       score[row] = rk::Elem<T>::get(r[y]);
     else if (p == 0 && (y < 0 || y >= a.V))
@@ -70,11 +83,11 @@ __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__r
     for (int e = 0; e < n; ++e) sum += __expf(f[e] - m);
   };
   const int32_t steps = (hi - lo) / kStep;
-  const T *q = r + lo + (int)threadIdx.x * VEC;
+  const T *q = r + lo + lane * VEC;
   rk::Pack<T, VEC> v[U];
   if (steps > 0)
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u].load(q + u * kThreads * VEC);
+    for (int u = 0; u < U; ++u) v[u].load(q + u * TPR * VEC);
   for (int32_t k = 0; k < steps; ++k) {
     float f[U * VEC];
 #pragma unroll
@@ -82,16 +95,16 @@ __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__r
     q += kStep;
     if (k + 1 < steps)
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u].load(q + u * kThreads * VEC);
+      for (int u = 0; u < U; ++u) v[u].load(q + u * TPR * VEC);
     add(f, U * VEC);
   }
   // the rest of the part: less than one step
-  int32_t j = lo + steps * kStep + (int32_t)threadIdx.x * VEC;
+  int32_t j = lo + steps * kStep + lane * VEC;
 #pragma unroll
   for (int u = 0; u < U; ++u)
-    if (j + u * kThreads * VEC + VEC <= hi) v[u].load(r + j + u * kThreads * VEC);
+    if (j + u * TPR * VEC + VEC <= hi) v[u].load(r + j + u * TPR * VEC);
 #pragma unroll
-  for (int u = 0; u < U; ++u, j += kThreads * VEC) {
+  for (int u = 0; u < U; ++u, j += TPR * VEC) {
     float f[VEC];
     if (j + VEC <= hi) {
       v[u].widen(f);
@@ -107,6 +120,10 @@ __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__r
     const float om = __shfl_xor(m, off, rk::kWave), os = __shfl_xor(sum, off, rk::kWave);
     merge(m, sum, om, os);
   }
+  if constexpr (TPR == rk::kWave) {
+    if (lane == 0) part[unit] = make_float2(m, sum);
+    return;
+  }
   if (threadIdx.x % rk::kWave == 0) {
     s_m[threadIdx.x / rk::kWave] = m;
     s_s[threadIdx.x / rk::kWave] = sum;
@@ -115,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void rows_fwd_kernel(Rows a, const T *__r
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) merge(m, sum, s_m[w], s_s[w]);
-    part[blockIdx.x] = make_float2(m, sum);
+    part[unit] = make_float2(m, sum);
   }
 }
 
@@ -276,18 +293,20 @@ __global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float
 // last row to the first: those were read last and some of them are still cached.  ONCE: a gradient that
 // is larger than what the caches should hold is stored past them (left there, its 403 MB were written
 // back under the next call's forward launch, which took 74 us instead of 41).
-template <typename T, bool ONCE>
+template <typename T, int TPR, bool ONCE>
 __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__restrict__ x, const float2 *__restrict__ stat,
                                                             const float *__restrict__ g_loss, const float *__restrict__ slope,
                                                             const float *__restrict__ g_logps, int average,
                                                             const int32_t *__restrict__ used, T *__restrict__ dx) {
   constexpr int VEC = rk::Elem<T>::kVec, U = 4;
-  const uint32_t block = gridDim.x - 1 - blockIdx.x;
-  const int64_t row = block / a.parts;
-  const int32_t p = (int32_t)(block - row * a.parts), s = (int32_t)(row / a.T), t = (int32_t)(row - (int64_t)s * a.T);
+  const uint32_t from_end = unit_index<TPR>();
+  if (from_end >= a.units) return;
+  const uint32_t unit = a.units - 1 - from_end, row = unit / (uint32_t)a.parts;
+  const int lane = TPR == kThreads ? threadIdx.x : threadIdx.x % TPR;
+  const int32_t p = (int32_t)(unit - row * a.parts), s = (int32_t)(row / (uint32_t)a.T), t = (int32_t)(row - (uint32_t)s * a.T);
   const int32_t lo = p * a.part_len, hi = min(a.V, lo + a.part_len);
   const int64_t y = a.items[s * a.ld_items + t];
-  T *d = dx + row * a.V;
+  T *d = dx + (int64_t)row * a.V;
   auto put = [&](const rk::Pack<T, VEC> &o, int32_t j) {
     if constexpr (ONCE)
       o.store_once(d + j);
@@ -298,7 +317,7 @@ __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__r
     rk::Pack<T, VEC> zero;
 #pragma unroll
     for (int i = 0; i < rk::Pack<T, VEC>::kWords; ++i) zero.w[i] = 0u;
-    for (int32_t j = lo + (int32_t)threadIdx.x * VEC; j < hi; j += kThreads * VEC) {
+    for (int32_t j = lo + lane * VEC; j < hi; j += TPR * VEC) {
       if (j + VEC <= hi) {
         put(zero, j);
       } else {
@@ -327,15 +346,15 @@ __global__ __launch_bounds__(kThreads) void rows_bwd_kernel(Rows a, const T *__r
     o.narrow(f);
     put(o, j);
   };
-  int32_t j = lo + (int32_t)threadIdx.x * VEC;
-  for (; j + (U - 1) * kThreads * VEC + VEC <= hi; j += U * kThreads * VEC) {
+  int32_t j = lo + lane * VEC;
+  for (; j + (U - 1) * TPR * VEC + VEC <= hi; j += U * TPR * VEC) {
     rk::Pack<T, VEC> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u].load(r + j + u * kThreads * VEC);
+    for (int u = 0; u < U; ++u) v[u].load(r + j + u * TPR * VEC);
 #pragma unroll
-    for (int u = 0; u < U; ++u) one(v[u], j + u * kThreads * VEC);
+    for (int u = 0; u < U; ++u) one(v[u], j + u * TPR * VEC);
   }
-  for (; j < hi; j += kThreads * VEC) {
+  for (; j < hi; j += TPR * VEC) {
     if (j + VEC <= hi) {
       rk::Pack<T, VEC> v;
       v.load(r + j);
@@ -360,6 +379,19 @@ void cut(Rows &a, int want_blocks) {
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>(rk::ceil_div(want_blocks, rows), rk::ceil_div(a.V, kMinPart)));
   a.part_len = (int32_t)(rk::ceil_div(rk::ceil_div(a.V, want), 8) * 8);
   a.parts = (int32_t)rk::ceil_div(a.V, a.part_len);
+  a.units = (uint32_t)std::min<int64_t>(rows * a.parts, INT32_MAX);
+}
+
+// Up to this many scores a wavefront takes a part.  Microseconds for bf16 rows, by a wavefront / by a workgroup:
+// forward 94 / 294 (200000 rows of 100 scores), 47 / 126 (100000 of 1000), 38 / 52 (30000 of 4000), 6.0 / 7.2
+// (2000 of 4000); backward 73 / 186, 61 / 96, 4.5 / 5.2 (2000 of 1000), 7.1 / 5.8 (2000 of 2000).
+constexpr int kWaveFwd = 4096, kWaveBwd = 1024;
+// (few parts: the longer ones by a workgroup, 4.0 us instead of 4.4 for 16 parts of 3525)
+bool fwd_by_wave(const Rows &a) { return a.part_len <= (a.units >= 1024 ? kWaveFwd : kWaveFwd / 2); }
+
+dim3 grid_of(const Rows &a, bool by_wave) {
+  const int64_t blocks = rk::ceil_div((int64_t)a.units, by_wave ? kWaves : 1), x = std::min<int64_t>(blocks, 1 << 22);
+  return dim3((uint32_t)x, (uint32_t)rk::ceil_div(blocks, x));
 }
 
 int make_rows(Rows &a, int32_t dtype, int32_t S, int32_t T, int32_t V, int64_t stride_s, int64_t stride_t,
@@ -368,11 +400,11 @@ int make_rows(Rows &a, int32_t dtype, int32_t S, int32_t T, int32_t V, int64_t s
   RK_CHECK_ARG(S >= 0 && T >= 0 && V >= 1, "bad size: %d lists, %d places, %d items", S, T, V);
   // a part's last step may look a few thousand scores past its end before it stops
   RK_CHECK_ARG(V < (1 << 30), "more than 2^30 items");
-  a = {stride_s, stride_t, S, T, V, 0, 0, items, ld_items, ignore};
+  a = {stride_s, stride_t, S, T, V, 0, 0, items, ld_items, ignore, 0};
   if (S == 0 || T == 0) return RK_OK;
   RK_CHECK_ARG(items, "null pointer");
   cut(a, want_blocks);
-  RK_CHECK_ARG((int64_t)S * T * a.parts < INT32_MAX, "too many rows");
+  RK_CHECK_ARG((int64_t)S * T * a.parts < INT32_MAX, "too many rows for one call");
   return RK_OK;
 }
 
@@ -389,8 +421,10 @@ Ws ws_of(const Rows &a) {
 
 template <typename T>
 int launch_rows_fwd(const Rows &a, const void *x, float *ws, const Ws &w, hipStream_t st) {
-  rows_fwd_kernel<T><<<(uint32_t)((int64_t)a.S * a.T * a.parts), kThreads, 0, st>>>(a, (const T *)x, (float2 *)(ws + w.part),
-                                                                                  ws + w.score);
+  if (fwd_by_wave(a))
+    rows_fwd_kernel<T, rk::kWave><<<grid_of(a, true), kThreads, 0, st>>>(a, (const T *)x, (float2 *)(ws + w.part), ws + w.score);
+  else
+    rows_fwd_kernel<T, kThreads><<<grid_of(a, false), kThreads, 0, st>>>(a, (const T *)x, (float2 *)(ws + w.part), ws + w.score);
   RK_CHECK_LAUNCH("rows_fwd_kernel");
   return RK_OK;
 }
@@ -439,13 +473,21 @@ constexpr int64_t kStreamBytes = 64 << 20;   // gradients from this size on are 
 template <typename T>
 int run_bwd(const Rows &a, const void *x, const float *stat, const float *g_loss, const float *slope, const float *g_logps,
             int average, const int32_t *used, void *dx, hipStream_t st) {
-  const uint32_t blocks = (uint32_t)((int64_t)a.S * a.T * a.parts);
-  if ((int64_t)a.S * a.T * a.V * (int64_t)sizeof(T) >= kStreamBytes)
-    rows_bwd_kernel<T, true><<<blocks, kThreads, 0, st>>>(a, (const T *)x, (const float2 *)stat, g_loss, slope, g_logps, average,
-                                                        used, (T *)dx);
-  else
-    rows_bwd_kernel<T, false><<<blocks, kThreads, 0, st>>>(a, (const T *)x, (const float2 *)stat, g_loss, slope, g_logps,
-                                                         average, used, (T *)dx);
+  const bool once = (int64_t)a.S * a.T * a.V * (int64_t)sizeof(T) >= kStreamBytes;
+#define RK_BWD(TPR, ONCE)                                                                                             \
+  rows_bwd_kernel<T, TPR, ONCE><<<grid_of(a, TPR == rk::kWave), kThreads, 0, st>>>(a, (const T *)x, (const float2 *)stat, g_loss, slope, \
+                                                                 g_logps, average, used, (T *)dx)
+  if (a.part_len <= kWaveBwd) {
+    if (once)
+      RK_BWD(rk::kWave, true);
+    else
+      RK_BWD(rk::kWave, false);
+  } else if (once) {
+    RK_BWD(kThreads, true);
+  } else {
+    RK_BWD(kThreads, false);
+  }
+#undef RK_BWD
   RK_CHECK_LAUNCH("rows_bwd_kernel");
   return RK_OK;
 }
@@ -456,7 +498,7 @@ extern "C" {
 
 size_t rk_list_logps_ws_bytes(int32_t S, int32_t T, int32_t V) {
   if (S <= 0 || T <= 0 || V <= 0) return 0;
-  Rows a = {0, 0, S, T, V, 0, 0, nullptr, 0, 0};
+  Rows a = {0, 0, S, T, V, 0, 0, nullptr, 0, 0, 0};
   cut(a, kWantFwd);
   return (size_t)ws_of(a).words * 4;
 }
