@@ -18,7 +18,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
-#include <cmath>
+#include <mutex>
 
 #include "../../include/recommend_amd.h"
 
@@ -91,6 +91,10 @@ Tensor scratch(size_t bytes, const Tensor &like) {
 
 bool records(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
+void no_tangent(const char *what, const Tensor &t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // Gradients for a graph of the gradient (create_graph): they depend on what this node does not differentiate,
 // so differentiating them raises.
 variable_list only_once(const char *what, variable_list grads) {
@@ -111,12 +115,19 @@ struct LookupBackward : public Node {
   int32_t kind = 0;
 
   std::string name() const override { return "EmbeddingLookupBackward"; }
-  void release_variables() override { ids_.reset_data(); }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ids_.reset_data();
+  }
 
-  Tensor gradient(const Tensor &grad, const Tensor &ids) {
-    const Tensor g = grad.contiguous();
+  Tensor gradient(const Tensor &grad, const Tensor &ids_in) {
+    const Tensor g = grad.contiguous(), ids = ids_in.contiguous();
     c10::DeviceGuard guard(g.device());
     const int64_t n = ids.numel();
+    // (a hook on saved tensors may have put something else in their place)
+    TORCH_CHECK(n * D == g.numel() && ids.device() == g.device() &&
+                    (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+                "embedding_lookup: the saved ids are not those of the forward pass");
     Tensor dw = at::empty({rows, D}, g.options());
     const Tensor ws = scratch(abi.rk_embedding_bwd_ws_bytes(n, (int32_t)rows, (int32_t)D, kind), g);
     check_in_backward(abi.rk_embedding_bwd(g.data_ptr(), kind, ids.data_ptr(), (int32_t)ids.element_size(), n, (int32_t)rows,
@@ -126,9 +137,11 @@ struct LookupBackward : public Node {
   }
 
   variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     const Tensor &grad = grads[0];
     if (!grad.defined() || !task_should_compute_output(0)) return {Tensor()};
-    const Tensor ids = ids_.unpack(shared_from_this());
+    no_tangent("embedding_lookup", grad);
+    const Tensor ids = ids_.unpack();
     // (linear in the upstream gradient: its derivative matters only where that has one)
     const bool graph = at::GradMode::is_enabled() && grad.requires_grad();
     at::AutoGradMode off(false);
@@ -140,6 +153,7 @@ struct LookupBackward : public Node {
 };
 
 Tensor embedding_lookup(const Tensor &weight, const Tensor &ids_in, double scale, std::optional<int64_t> padding_idx) {
+  no_tangent("embedding_lookup", weight);
   TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) >= 1, "embedding_lookup: the table is [rows, D], got ", weight.sizes());
   const int32_t kind = elem_of(weight.scalar_type(), "embedding_lookup");
   const int64_t rows = weight.size(0), D = weight.size(1);
@@ -164,7 +178,7 @@ Tensor embedding_lookup(const Tensor &weight, const Tensor &ids_in, double scale
     auto shape = ids.sizes().vec();
     shape.push_back(D);
     out = at::empty(shape, w.options());
-    check(abi.rk_embedding_fwd(w.data_ptr(), w.stride(0), (int32_t)rows, (int32_t)D, kind, ids.data_ptr(),
+    check(abi.rk_embedding_fwd(w.data_ptr(), rows > 1 ? w.stride(0) : D, (int32_t)rows, (int32_t)D, kind, ids.data_ptr(),
                                (int32_t)ids.element_size(), ids.numel(), (float)scale, out.data_ptr(),
                                stream_of(w.device())));
   }
@@ -194,29 +208,48 @@ Geometry geometry_of(const Tensor &scores, int32_t kind) {
           places ? scores.stride(1) : 0};
 }
 
+// rows whose scores lie side by side
+Tensor rows_in_order(const Tensor &scores) {
+  return scores.stride(-1) == 1 || scores.size(-1) == 1 ? scores : scores.contiguous();
+}
+
 struct ListBackward : public Node {
   SavedVariable scores_, items_;
+  std::vector<int64_t> shape_;
+  at::ScalarType type_ = at::kFloat;
   Tensor keep;                        // (max, log sum) of the rows, used places and slopes of the lists
-  Geometry geo;
   int64_t ignore = 0;
-  int32_t average = 0;
+  int32_t average = 0, kind = 0;
   bool pairs = false;
 
   std::string name() const override { return pairs ? "PreferenceLossBackward" : "ListLogpsBackward"; }
   void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
     scores_.reset_data();
     items_.reset_data();
     keep.reset();
   }
 
   variable_list apply(variable_list &&grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    const char *what = pairs ? "preference_loss" : "list_logps";
+    for (const Tensor &g : grads)
+      if (g.defined()) no_tangent(what, g);
     const Tensor g_logps = grads[0].defined() ? grads[0].detach() : Tensor();
     const Tensor g_loss = grads.size() > 1 && grads[1].defined() ? grads[1].detach() : Tensor();
     if ((!g_logps.defined() && !g_loss.defined()) || !task_should_compute_output(0)) return {Tensor()};
-    const Tensor scores = scores_.unpack(), items = items_.unpack();
+    Tensor scores = scores_.unpack(), items = items_.unpack();
     const bool graph = at::GradMode::is_enabled();
     at::AutoGradMode off(false);
     c10::DeviceGuard guard(scores.device());
+    // (a hook on saved tensors, one that keeps them on the host for example, gives back other strides)
+    scores = rows_in_order(scores);
+    items = items.contiguous();
+    const Geometry geo = geometry_of(scores, kind);
+    TORCH_CHECK(scores.sizes() == shape_ && scores.scalar_type() == type_ && items.scalar_type() == at::kLong &&
+                    items.numel() == (int64_t)geo.S * geo.T && items.device() == scores.device() &&
+                    (geo.S == 0 || keep.device() == scores.device()),
+                what, ": the saved tensors are not those of the forward pass");
     Tensor dx = at::empty(scores.sizes(), scores.options().memory_format(at::MemoryFormat::Contiguous));
     if (geo.S > 0) {
       const Tensor gp = g_logps.defined() ? g_logps.to(at::kFloat).contiguous() : Tensor();
@@ -230,13 +263,14 @@ struct ListBackward : public Node {
     }
     if (!graph) return {dx};
     at::AutoGradMode on(true);
-    return only_once(pairs ? "preference_loss" : "list_logps", {dx});
+    return only_once(what, {dx});
   }
 };
 
 // the loss where ref is given (undefined otherwise), and the lists' log-probabilities
 std::pair<Tensor, Tensor> lists(const char *what, const Tensor &scores_in, const Tensor &items_in, const Tensor &ref_in,
                                 int64_t ignore, bool average, double beta, double smoothing, int32_t form) {
+  no_tangent(what, scores_in);
   const int32_t kind = elem_of(scores_in.scalar_type(), what);
   TORCH_CHECK_VALUE(items_in.scalar_type() == at::kLong || items_in.scalar_type() == at::kInt, what,
                     ": items are int32 or int64, not ", c10::toString(items_in.scalar_type()));
@@ -252,7 +286,7 @@ std::pair<Tensor, Tensor> lists(const char *what, const Tensor &scores_in, const
   c10::DeviceGuard guard(scores_in.device());
   const bool record = records(scores_in);
   // (recorded: the gradient of a copy finds its way back)
-  const Tensor scores = scores_in.stride(-1) == 1 || scores_in.size(-1) == 1 ? scores_in : scores_in.contiguous();
+  const Tensor scores = rows_in_order(scores_in);
   const Geometry geo = geometry_of(scores, kind);
   Tensor items, keep, logps, loss;
   {
@@ -287,7 +321,9 @@ std::pair<Tensor, Tensor> lists(const char *what, const Tensor &scores_in, const
     node->scores_ = SavedVariable(scores, false);
     node->items_ = SavedVariable(items, false);
     node->keep = keep;
-    node->geo = geo;
+    node->shape_ = scores.sizes().vec();
+    node->type_ = scores.scalar_type();
+    node->kind = kind;
     node->ignore = ignore;
     node->average = average;
     node->pairs = loss.defined();

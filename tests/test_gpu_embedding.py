@@ -143,6 +143,25 @@ def test_views_of_tables_and_gradients(dtype):
             check(view, ids, grad, 0.5, None, out, dw)
 
 
+def test_saved_ids_that_were_kept_on_the_host():
+    w = torch.randn(50, 8, device=DEV, requires_grad=True)
+    ids = torch.randint(50, (6, 7), device=DEV)
+    want, = torch.autograd.grad(ops.embedding_lookup(w, ids).square().sum(), w)
+    with torch.autograd.graph.save_on_cpu():
+        loss = ops.embedding_lookup(w, ids).square().sum()
+    assert torch.equal(torch.autograd.grad(loss, w)[0], want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:2]):
+        out = ops.embedding_lookup(w, ids)
+    with pytest.raises(RuntimeError, match="not those of the forward pass"):
+        out.sum().backward()
+
+
+def test_a_table_of_one_row_with_any_stride():
+    w = torch.randn(8, device=DEV)
+    one = torch.as_strided(w, (1, 8), (0, 1))
+    assert torch.equal(ops.embedding_lookup(one, torch.zeros(3, dtype=torch.long, device=DEV)), w.expand(3, 8))
+
+
 def test_gradient_against_differences():
     g = torch.Generator().manual_seed(3)
     weight = torch.randn(30, 20, generator=g).to(DEV)

@@ -77,7 +77,7 @@ def make(S, T, V, dtype, seed, spread=3.0):
 
 
 SHAPES = [(2, 1, 1), (2, 1, 2), (4, 3, 7), (6, 2, 63), (2, 70, 65), (4, 5, 1000), (2, 2, 4097), (8, 3, 7050), (2, 1, 63001),
-          (2, 300, 129), (34, 1, 515)]
+          (2, 300, 129), (34, 1, 515), (6, 3, 1024), (6, 3, 1025), (6, 3, 2047), (6, 3, 2049)]
 
 
 @pytest.mark.parametrize("S,T,V", SHAPES)
@@ -221,6 +221,25 @@ def test_strided_scores(dtype):
         assert torch.equal(*(torch.autograd.grad(l, s)[0].contiguous() for l, s in ((la, a), (lb, b))))
     wide = items.repeat(1, 2)[:, ::2]                                  # strided and 32-bit items
     assert torch.equal(list_logps(big[:4, :5], wide), list_logps(big[:4, :5], wide.to(torch.int32)))
+
+
+def test_saved_tensors_that_were_kept_on_the_host():
+    """They come back with other strides than they had."""
+    g = torch.Generator().manual_seed(18)
+    big = torch.randn(8, 6, 301, generator=g).to(DEV)
+    items, ref = torch.randint(300, (4, 5), generator=g).to(DEV), torch.zeros(4, device=DEV)
+    for view in (big[::2, 1:, 1:], big[:1, :5].expand(4, 5, 301), big[:4, :5, ::2]):
+        it = items.clamp_max(view.shape[2] - 1)
+        a = view.detach().requires_grad_(True)
+        want, = torch.autograd.grad(preference_loss(a, it, ref)[0], a)
+        with torch.autograd.graph.save_on_cpu():
+            loss, _ = preference_loss(a, it, ref)
+        got, = torch.autograd.grad(loss, a)
+        assert torch.equal(got, want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:2]):
+        loss, _ = preference_loss(a, it, ref)
+    with pytest.raises(RuntimeError, match="not those of the forward pass"):
+        loss.backward()
 
 
 def test_lists_of_one_item_without_a_place_axis():
