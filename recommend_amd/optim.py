@@ -192,6 +192,11 @@ def decode_moment(code, scale, like):
     return (code.float().view(-1, _ffi.ADAMW_BLOCK) * scale.unsqueeze(1)).view(-1)[:like.numel()].view(like.shape)
 
 
+def _not_in_a_capture():
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """AdamW (the reference trainer's other choice, train/graph_trainer.py:78-101) with
     clip_grad_norm_ on the library's fused step (rk_adamw_step), over all parameter groups at once.
@@ -206,8 +211,9 @@ class FusedAdamW(torch.optim.Optimizer):
     `exp_avg8_scale`, `exp_avg_sq8`, `exp_avg_sq8_scale`): 2.1 bytes for each element instead of 8.
 
     As with FusedClipAdam the step count and the learning rates live in device memory, a step can be
-    recorded in a HIP graph after one eager step, and parameters without a gradient take no part.
-    Checkpoints load across state_bits and from torch.optim.AdamW."""
+    recorded in a HIP graph after one eager step, and parameters without a gradient take no part.  The
+    step count is one for all parameters.  Parameters must not share memory (one object given twice in a group
+    is refused).  Checkpoints load across state_bits and from torch.optim.AdamW."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,
                  state_bits=32, min_8bit_size=4096):
@@ -220,12 +226,20 @@ class FusedAdamW(torch.optim.Optimizer):
         self._dev = None
         self._rates = None       # learning rates that lr_dev holds
         self._ws = None
+        self._held = []
         self._restored_step = None
         self.grad_norm = None    # device scalar: total gradient norm of the last clipped step, before clipping
 
     def add_param_group(self, group):
         if len(self.param_groups) >= _ffi.ADAMW_MAX_GROUPS:
             raise ValueError(f"FusedAdamW takes up to {_ffi.ADAMW_MAX_GROUPS} parameter groups")
+        params = group["params"]
+        if not torch.is_tensor(params) and not isinstance(params, set):
+            params = list(params)
+            # (a parameter given twice would be updated by two workgroups at once)
+            if len({id(p[1] if isinstance(p, tuple) else p) for p in params}) != len(params):
+                raise ValueError("FusedAdamW: a parameter appears twice in a group")
+            group = {**group, "params": params}
         super().add_param_group(group)
         g = self.param_groups[-1]
         b1, b2 = g["betas"]
@@ -241,11 +255,13 @@ class FusedAdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         if "_dev" not in self.__dict__:      # a copy or an unpickled optimizer: device scalars are made anew
             self._dev = self._rates = self._ws = self.grad_norm = None
+            self._held = []
 
     def _is8(self, p):
         return self.state_bits == 8 and p.numel() >= self.min_8bit_size
 
     def _state_for(self, p):
+        _not_in_a_capture()      # (a replay would start the moments from zero every time)
         st = self.state[p]
         if self._is8(p):
             if "exp_avg8" not in st:
@@ -286,12 +302,13 @@ class FusedAdamW(torch.optim.Optimizer):
                 return loss
             if not first.is_cuda:
                 self._refuse(first, first.grad)
+            _not_in_a_capture()
             self._init_device(first.device)
         self.sync_lr()
         need = self._launch()
         if need:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
+            _not_in_a_capture()
+            self._held.append(self._ws)      # a recorded step goes on with the one that it was recorded with
             self._ws = torch.empty(need // 8, dtype=torch.float64, device=self._dev)
             self._launch()
         return loss

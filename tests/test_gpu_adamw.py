@@ -288,6 +288,54 @@ def test_recorded_in_a_graph_and_replayed(bits):
         assert all(torch.equal(p, q) for p, q in zip(ours, eager)) and int(a.step_count) == int(b.step_count) == k + 2
 
 
+def test_recorded_step_outlives_a_larger_workspace():
+    """A step over one tensor is recorded; later steps over more tensors need a larger workspace.  The recorded step
+    goes on with its own, which nothing else has been given meanwhile."""
+    first, more = params_of([(300, 64)], torch.Generator().manual_seed(16))[0], [torch.nn.Parameter(torch.zeros(8, device=DEV))
+                                                                               for _ in range(60)]
+    opt = FusedAdamW([first] + more, lr=1e-2, max_grad_norm=1.0)
+    first.grad = torch.ones_like(first)
+    opt.step()
+    size = opt._ws.numel()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for p in more:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert opt._ws.numel() > size
+    others = [torch.full((size,), 7.0, dtype=torch.float64, device=DEV) for _ in range(20)]
+    twin = torch.nn.Parameter(first.detach().clone())
+    same = FusedAdamW([twin], lr=1e-2, max_grad_norm=1.0)
+    twin.grad = first.grad
+    same.load_state_dict({"state": {0: {k: v.clone() for k, v in opt.state[first].items()} | {"step": 2}},
+                          "param_groups": same.state_dict()["param_groups"]})
+    for _ in range(3):
+        graph.replay()
+        same.step()
+        torch.cuda.synchronize()
+        assert torch.equal(first, twin)
+    assert all(bool((o == 7.0).all()) for o in others)
+
+
+def test_a_first_step_is_not_recorded():
+    a, b = params_of([(300, 64), (64,)], torch.Generator().manual_seed(17))
+    opt = FusedAdamW([a, b], lr=1e-2)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    for missing in (2, 1):                               # both parameters' moments, then one's
+        before = [p.detach().clone() for p in (a, b)]
+        with pytest.raises(RuntimeError, match="before capturing"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+        assert torch.equal(a, before[0]) and torch.equal(b, before[1])
+        if missing == 2:
+            b.grad = None
+            opt.step()
+            b.grad = torch.ones_like(b)
+    opt.step()
+    assert int(opt.step_count) == 2
+
+
 def test_refuses_what_it_cannot_update():
     opt = FusedAdamW([torch.nn.Parameter(torch.zeros(8, 8, device=DEV).t()[1:])])
     p = opt.param_groups[0]["params"][0]
@@ -303,6 +351,21 @@ def test_refuses_what_it_cannot_update():
     r.grad = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.ones(1, 4), (8, 4)).to(DEV)
     with pytest.raises(_ffi.RkError, match="dense"):
         FusedAdamW([r]).step()
+
+
+def test_state_of_other_sizes_is_refused():
+    for bits in (8, 32):
+        p = torch.nn.Parameter(torch.zeros(5000, device=DEV))
+        p.grad = torch.ones_like(p)
+        opt = FusedAdamW([p], state_bits=bits)
+        opt.step()
+        key = "exp_avg8" if bits == 8 else "exp_avg"
+        for bad in (opt.state[p][key][:-64], opt.state[p][key].float().half(), opt.state[p][key].cpu()):
+            keep, opt.state[p][key] = opt.state[p][key], bad
+            with pytest.raises(ValueError, match="not what this optimizer made"):
+                opt.step()
+            opt.state[p][key] = keep
+        opt.step()
 
 
 def test_the_same_step_as_clip_adam_without_decay():

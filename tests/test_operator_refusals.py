@@ -73,11 +73,27 @@ def test_adamw_refuses():
         FusedAdamW([p()], weight_decay=-0.1)
     with pytest.raises(ValueError, match="up to 8"):
         FusedAdamW([{"params": [p()]} for _ in range(9)])
+    twice = p()
+    with pytest.raises(ValueError, match="twice"):
+        FusedAdamW([twice, p(), twice])
+    with pytest.raises(ValueError, match="twice"):
+        FusedAdamW([{"params": iter([twice, twice])}])
     opt = FusedAdamW([p()])
     opt.step()                                            # no gradient: nothing to do
     opt.param_groups[0]["params"][0].grad = F(4)
     with pytest.raises(_ffi.RkError, match="HIP device"):
         opt.step()
+
+
+def test_forward_derivatives_are_refused():
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda *shape: torch.autograd.forward_ad.make_dual(F(*shape), F(*shape))  # noqa: E731
+        with pytest.raises(NotImplementedError, match="embedding_lookup has no forward-mode"):
+            ops.embedding_lookup(dual(4, 8), long(3))
+        with pytest.raises(NotImplementedError, match="list_logps has no forward-mode"):
+            ops.list_logps(dual(2, 3, 5), long(2, 3))
+        with pytest.raises(NotImplementedError, match="preference_loss has no forward-mode"):
+            preference_loss(dual(2, 3, 5), long(2, 3), F(2))
 
 
 def refused(name, *args, error=""):
