@@ -192,6 +192,9 @@ def decode_moment(code, scale, like):
     return (code.float().view(-1, _ffi.ADAMW_BLOCK) * scale.unsqueeze(1)).view(-1)[:like.numel()].view(like.shape)
 
 
+_NEVER = 2 ** 62        # elements that no tensor has
+
+
 def _not_in_a_capture():
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("run one optimizer step with these parameters before capturing it in a graph")
@@ -260,20 +263,6 @@ class FusedAdamW(torch.optim.Optimizer):
     def _is8(self, p):
         return self.state_bits == 8 and p.numel() >= self.min_8bit_size
 
-    def _state_for(self, p):
-        _not_in_a_capture()      # (a replay would start the moments from zero every time)
-        st = self.state[p]
-        if self._is8(p):
-            if "exp_avg8" not in st:
-                blocks = -(-p.numel() // _ffi.ADAMW_BLOCK)
-                for k in ("exp_avg8", "exp_avg_sq8"):
-                    st[k] = torch.zeros(blocks * _ffi.ADAMW_BLOCK, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn)
-                    st[k + "_scale"] = torch.zeros(blocks, dtype=torch.float32, device=p.device)
-        elif "exp_avg" not in st:
-            for k in _STATE32:
-                st[k] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-        return st
-
     def _init_device(self, dev):
         self._dev = dev
         if self._restored_step is None:
@@ -281,7 +270,8 @@ class FusedAdamW(torch.optim.Optimizer):
         self.step_count = torch.full((1,), self._restored_step, dtype=torch.int64, device=dev)
         self.lr_dev = torch.zeros(_ffi.ADAMW_MAX_GROUPS, dtype=torch.float32, device=dev)
         self.grad_norm = torch.zeros(1, dtype=torch.float32, device=dev)
-        self._ws = torch.empty(0, dtype=torch.float64, device=dev)
+        tensors = sum(len(g["params"]) for g in self.param_groups)
+        self._ws = torch.empty(_ffi.load().rk_adamw_ws_bytes(tensors) // 8, dtype=torch.float64, device=dev)
 
     def _refuse(self, p, g):
         if not p.is_cuda:
@@ -314,8 +304,11 @@ class FusedAdamW(torch.optim.Optimizer):
         return loss
 
     def _launch(self):
-        return _ffi.torch_ops().adamw_step(self.param_groups, self.state, self._state_for, self._refuse, self.step_count,
-                                           self.lr_dev, self.max_grad_norm or 0.0, self.grad_norm, self._ws)
+        # (moments that a capture made would start from zero at every replay)
+        return _ffi.torch_ops().adamw_step(self.param_groups, self.state,
+                                           self.min_8bit_size if self.state_bits == 8 else _NEVER, _not_in_a_capture,
+                                           self._refuse, self.step_count, self.lr_dev, self.max_grad_norm or 0.0,
+                                           self.grad_norm, self._ws)
 
     def sync_lr(self):
         """Push learning rates changed by a scheduler to device memory (step() does it; call it for a step that

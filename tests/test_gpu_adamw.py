@@ -293,13 +293,14 @@ def test_recorded_step_outlives_a_larger_workspace():
     goes on with its own, which nothing else has been given meanwhile."""
     first, more = params_of([(300, 64)], torch.Generator().manual_seed(16))[0], [torch.nn.Parameter(torch.zeros(8, device=DEV))
                                                                                for _ in range(60)]
-    opt = FusedAdamW([first] + more, lr=1e-2, max_grad_norm=1.0)
+    opt = FusedAdamW([first], lr=1e-2, max_grad_norm=1.0)
     first.grad = torch.ones_like(first)
     opt.step()
     size = opt._ws.numel()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         opt.step()
+    opt.add_param_group({"params": more})
     for p in more:
         p.grad = torch.ones_like(p)
     opt.step()
