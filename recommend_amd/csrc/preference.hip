@@ -22,6 +22,9 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / rk::kWave;
 constexpr int kPairThreads = 1024;
 constexpr int kFewRows = 4096;       // rows that one workgroup joins
+// Pairs that one workgroup adds up behind more rows than that; more take two launches (4096 pairs 7.2 us, in two
+// launches 2.9 + 1.8 and a gap; 100000 pairs 129 us, 4.9 + 4.7).
+constexpr int kOnePairs = 4096;
 
 // A row's part is read by a workgroup, or by a wavefront (four parts in a workgroup): a row of 1000 scores
 // keeps 125 of 256 threads busy once.
@@ -150,26 +153,27 @@ __device__ __forceinline__ float row_logp(const Rows &a, int64_t row, const floa
   return (score[row] - m) - lq;
 }
 
-// One wavefront for every list: its log-probability and the number of its places in use.
+// The lists' log-probabilities and the numbers of their places in use.  `lanes` threads for a list: a power of two up
+// to 64 (200000 lists of one place: 5.1 us, by a wavefront each 51).
 __global__ __launch_bounds__(kThreads) void lists_kernel(Rows a, const float2 *__restrict__ part,
                                                          const float *__restrict__ score, float2 *__restrict__ stat,
-                                                         int average, float *__restrict__ logps,
+                                                         int average, int lanes, float *__restrict__ logps,
                                                          int32_t *__restrict__ used) {
-  const int32_t s = (int32_t)blockIdx.x * kWaves + threadIdx.x / rk::kWave;
+  const int64_t s = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
+  const int lane = (int)threadIdx.x & (lanes - 1);
   if (s >= a.S) return;
   double sum = 0.0;
   int32_t n = 0;
-  for (int32_t t = threadIdx.x % rk::kWave; t < a.T; t += rk::kWave) {
+  for (int32_t t = lane; t < a.T; t += lanes) {
     if (a.items[s * a.ld_items + t] == a.ignore) continue;
-    sum += (double)row_logp(a, (int64_t)s * a.T + t, part, score, stat);
+    sum += (double)row_logp(a, s * a.T + t, part, score, stat);
     ++n;
   }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
+  for (int off = lanes / 2; off > 0; off >>= 1) {
     sum += __shfl_xor(sum, off, rk::kWave);
     n += __shfl_xor(n, off, rk::kWave);
   }
-  if (threadIdx.x % rk::kWave == 0) {
+  if (lane == 0) {
     logps[s] = (float)(average && n > 0 ? sum / n : sum);
     used[s] = n;
   }
@@ -278,6 +282,44 @@ __global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float
     slope_out[p] = slope / (float)P;
     slope_out[P + p] = -slope / (float)P;
   }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, rk::kWave);
+  if (threadIdx.x % rk::kWave == 0) s_sum[threadIdx.x / rk::kWave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = s_sum[0];
+    for (int w = 1; w < kPairThreads / rk::kWave; ++w) all += s_sum[w];
+    loss[0] = (float)(all / P);
+  }
+}
+
+// Many pairs: their terms and slopes, and one partial sum for every workgroup ...
+__global__ __launch_bounds__(kThreads) void terms_kernel(int32_t P, const float *__restrict__ logps, const float *__restrict__ ref,
+                                                         float beta, float eps, int kind, float *__restrict__ slope_out,
+                                                         double *__restrict__ partial) {
+  __shared__ double s_sum[kWaves];
+  const int32_t p = (int32_t)blockIdx.x * kThreads + threadIdx.x;
+  double sum = 0.0;
+  if (p < P) {
+    float slope;
+    sum = (double)pair_term((logps[p] - ref[p]) - (logps[P + p] - ref[P + p]), beta, eps, kind, slope);
+    slope_out[p] = slope / (float)P;
+    slope_out[P + p] = -slope / (float)P;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, rk::kWave);
+  if (threadIdx.x % rk::kWave == 0) s_sum[threadIdx.x / rk::kWave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+}
+
+// ... and their mean, by one workgroup.
+__global__ __launch_bounds__(kPairThreads) void mean_kernel(int32_t P, const double *__restrict__ partial, int32_t n,
+                                                            float *__restrict__ loss) {
+  __shared__ double s_sum[kPairThreads / rk::kWave];
+  double sum = 0.0;
+#pragma unroll 8
+  for (int32_t i = threadIdx.x; i < n; i += kPairThreads) sum += partial[i];
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, rk::kWave);
   if (threadIdx.x % rk::kWave == 0) s_sum[threadIdx.x / rk::kWave] = sum;
@@ -431,8 +473,12 @@ int launch_rows_fwd(const Rows &a, const void *x, float *ws, const Ws &w, hipStr
 
 int launch_lists(const Rows &a, int average, float *stat, float *logps, int32_t *used, const float *ws, const Ws &w,
                  hipStream_t st) {
-  lists_kernel<<<(uint32_t)rk::ceil_div(a.S, kWaves), kThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score,
-                                                                        (float2 *)stat, average, logps, used);
+  int lanes = 1;
+  while (lanes < rk::kWave && lanes < a.T) lanes *= 2;
+  const int64_t blocks = rk::ceil_div((int64_t)a.S, kThreads / lanes);
+  RK_CHECK_ARG(blocks < rk::kMaxBlocks256, "too many lists for one call");
+  lists_kernel<<<(uint32_t)blocks, kThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score, (float2 *)stat, average,
+                                                    lanes, logps, used);
   RK_CHECK_LAUNCH("lists_kernel");
   return RK_OK;
 }
@@ -461,6 +507,15 @@ int run_pairs(const Rows &a, const void *x, const float *ref, int average, float
     RK_PAIRS(kFewRows / kPairThreads);
   } else {
     if (int rc = launch_lists(a, average, stat, logps, used, ws, w, st)) return rc;
+    const int32_t P = a.S / 2, blocks = (int32_t)rk::ceil_div(P, kThreads);
+    if (P > kOnePairs) {
+      // (the parts are joined: the partial sums take their place)
+      terms_kernel<<<blocks, kThreads, 0, st>>>(P, logps, ref, beta, eps, kind, slope, (double *)ws);
+      RK_CHECK_LAUNCH("terms_kernel");
+      mean_kernel<<<1, kPairThreads, 0, st>>>(P, (const double *)ws, blocks, loss);
+      RK_CHECK_LAUNCH("mean_kernel");
+      return RK_OK;
+    }
     RK_PAIRS(0);
   }
 #undef RK_PAIRS

@@ -125,6 +125,15 @@ def test_preference_loss_vs_float64(kind, eps, S, T, V, dtype):
     assert bool((err <= slack).all()), float((err - slack).max())
 
 
+# more rows than one workgroup joins, up to and above the pairs that one adds up
+@pytest.mark.parametrize("kind,eps", [("sigmoid", 0.1), ("squared", 0.0)])
+@pytest.mark.parametrize("S,T,V,dtype", [(8192, 1, 5, torch.float32), (8194, 1, 5, torch.float16), (10002, 1, 41, torch.float32),
+                                         (16500, 3, 18, torch.bfloat16), (1000, 5, 30, torch.float32),
+                                         (66, 70, 33, torch.float32)])
+def test_many_lists_vs_float64(kind, eps, S, T, V, dtype):
+    test_preference_loss_vs_float64(kind, eps, S, T, V, dtype)
+
+
 def test_both_results_are_differentiable():
     """loss + a term on the preferred lists' own log-probabilities: the gradients add."""
     scores, items, ref = make(4, 3, 200, torch.float32, 9)
