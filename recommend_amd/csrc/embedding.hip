@@ -36,6 +36,7 @@ constexpr int32_t kFewRows = 1 << (32 - kFewBits);      // (key and position hav
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
 constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
 constexpr int kPerGroup = 32;         // sorted entries of a lane group
+constexpr int kJoinLanes = 64;       // lanes of a row in the closing launch, at most
 constexpr int kJoins = 4;             // workgroup borders that one workgroup of the closing launch looks at
 constexpr int64_t kStreamBytes = 64 << 20;   // looked-up rows from this size on are stored past the caches
 constexpr int kLongRun = 8;          // workgroup pieces of a row above which a whole workgroup joins them
@@ -540,14 +541,17 @@ __device__ __forceinline__ void add_pieces(const SumArgs &a, int32_t k0, int32_t
 // Rows that cross workgroups: the workgroup in which such a row begins has a tail piece, the ones it
 // goes on into have head pieces; they are added in that order.  One lane group per workgroup of the
 // summing launch; rows with many pieces are added by the whole workgroup, a consecutive share each.
+// Wide rows are cut into slices of kJoinLanes vectors (blockIdx.y), so that enough lane groups share
+// the pieces (one id 16384 times, rows of 4000 floats: 50 us instead of 587; slices of 32
+// vectors cost ordinary rows of 1024 floats 32 us instead of 20).
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict__ dW) {
+__global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, int32_t L, T *__restrict__ dW) {
   __shared__ float s_part[256 * VEC];
   __shared__ int32_t s_last[kJoins];                       // last workgroup of the row that begins in this one (0: none)
   __shared__ int32_t s_end;
-  const int per_block = a.G * a.per_group;
-  const int grp = threadIdx.x / a.L, l = threadIdx.x - grp * a.L;
-  const int borders = min(a.G, kJoins);
+  const int per_block = a.G * a.per_group, G = 256 / L;   // (of the summing launch; lane groups of this one)
+  const int grp = threadIdx.x / L, l = threadIdx.x - grp * L;
+  const int borders = min(G, kJoins);
   const int32_t b = (int32_t)blockIdx.x * borders + grp;
   int32_t last = 0;
   if (grp < borders && (int64_t)(b + 1) * per_block < a.n) {
@@ -591,8 +595,9 @@ __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict_
     __syncthreads();
   }
   if (grp < borders) last = s_last[grp];
-  for (int c0 = 0; c0 < a.D; c0 += a.L * VEC) {
-    const bool on = grp < a.G && c0 + l * VEC < a.D;
+  for (int64_t c = (int64_t)blockIdx.y * L * VEC; c < a.D; c += (int64_t)gridDim.y * L * VEC) {
+    const int c0 = (int)c;
+    const bool on = grp < G && c0 + l * VEC < a.D;
     const int col = min(c0 + l * VEC, a.D - VEC);
     if (on && last > 0 && last - b <= kLongRun) {
       float acc[VEC];
@@ -605,7 +610,7 @@ __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict_
     for (int j = 0; j < borders; ++j) {                  // (the same for every thread: barriers inside)
       const int32_t bj = (int32_t)blockIdx.x * borders + j, lj = s_last[j], pieces = lj - bj;
       if (lj == 0 || pieces <= kLongRun) continue;
-      const int32_t share = (pieces + a.G - 1) / a.G;
+      const int32_t share = (pieces + G - 1) / G;
       if (on) {
         float acc[VEC];
 #pragma unroll
@@ -621,9 +626,9 @@ __global__ __launch_bounds__(256) void emb_join_kernel(SumArgs a, T *__restrict_
         const float *p = a.pieces + ((int64_t)bj * 2 + 1) * a.D + col;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] = p[e];
-        for (int q = 0; q < a.G; ++q)
+        for (int q = 0; q < G; ++q)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[e] += s_part[(q * a.L + l) * VEC + e];
+          for (int e = 0; e < VEC; ++e) acc[e] += s_part[(q * L + l) * VEC + e];
         put_row<T, VEC>(dW + (int64_t)a.keys[(int64_t)(bj + 1) * per_block - 1] * a.D + col, acc, a.scale);
       }
       __syncthreads();
@@ -755,7 +760,9 @@ int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
   emb_sum_kernel<T, VEC><<<(uint32_t)blocks, 256, 0, st>>>(a, (const T *)g, (T *)dW);
   RK_CHECK_LAUNCH("emb_sum_kernel");
   if (a.blocks > 1) {
-    emb_join_kernel<T, VEC><<<(uint32_t)rk::ceil_div(a.blocks - 1, std::min(a.G, kJoins)), 256, 0, st>>>(a, (T *)dW);
+    const int L = std::min(a.L, kJoinLanes);
+    const uint32_t slices = (uint32_t)std::min<int64_t>(1024, rk::ceil_div((int64_t)a.D, L * VEC));
+    emb_join_kernel<T, VEC><<<dim3((uint32_t)rk::ceil_div(a.blocks - 1, std::min(256 / L, kJoins)), slices), 256, 0, st>>>(a, L, (T *)dW);
     RK_CHECK_LAUNCH("emb_join_kernel");
   }
   return RK_OK;
