@@ -34,7 +34,11 @@ constexpr int kTile = kSortThreads * kTileSteps;
 constexpr int kFewBits = 9, kFewIds = 1 << kFewBits;   // ids that every summing workgroup sorts itself: one launch
 constexpr int32_t kFewRows = 1 << (32 - kFewBits);      // (key and position have to fit a word)
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
-constexpr int kZeroRows = 256;        // rows looked up by one zeroing workgroup
+constexpr int kZeroRows = 256;        // rows that a zeroing workgroup looks up together
+// Blocks of them for a workgroup where there are more than the GPU holds at a time (summing launch of 2^20 ids in 30
+// million rows of 8 floats: 403 us with four blocks, 579 with one; in 2.2 million rows 53 and 67).
+constexpr int kZeroSteps = 4;
+constexpr int32_t kManyRows = 2048 * kZeroSteps * kZeroRows;
 constexpr int kPerGroup = 32;         // sorted entries of a lane group
 constexpr int kJoinLanes = 64;       // lanes of a row in the closing launch, at most
 constexpr int kJoins = 4;             // workgroup borders that one workgroup of the closing launch looks at
@@ -287,6 +291,7 @@ struct SumArgs {
   int32_t n, rows, D;
   int32_t L, G, per_group;      // lanes of a row, rows side by side in a workgroup, entries of a lane group
   int32_t blocks;               // workgroups that sum; the ones behind them zero
+  int32_t zero_steps;           // blocks of kZeroRows rows for each of those, 1 or kZeroSteps
   float scale;
   float *pieces;                // [blocks][2][D]: what a workgroup has of the row it begins / ends in
 };
@@ -317,6 +322,36 @@ __device__ __forceinline__ void zero_rows(int32_t z, bool absent, int32_t D, T *
   for (int i = lane; i < rk::kWave * per_row; i += rk::kWave) {
     const int r = i / per_row;
     if ((mask >> r) & 1) zero.store(dW + (row0 + r) * D + min((i - r * per_row) * VEC, D - VEC));
+  }
+}
+
+// The rows of `K` blocks of kZeroRows from block z on: zeros where no sorted key names them.  A thread's K
+// searches, chains of loads that wait for each other, run side by side.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void zero_absent(const SumArgs &a, int32_t z, T *__restrict__ dW) {
+  int32_t v[K], lo[K], len[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = (z + k) * kZeroRows + (int32_t)threadIdx.x;
+    lo[k] = 0;
+    len[k] = a.n;
+  }
+  for (int32_t left = a.n; left > 0; left >>= 1) {       // (a step leaves half of `len` at most)
+    int32_t key[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) key[k] = a.keys[min(lo[k] + (len[k] >> 1), a.n - 1)];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int32_t half = len[k] >> 1;
+      const bool up = len[k] > 0 && key[k] < v[k];
+      lo[k] = up ? lo[k] + half + 1 : lo[k];
+      len[k] = up ? len[k] - half - 1 : half;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const bool found = lo[k] < a.n && a.keys[min(lo[k], a.n - 1)] == v[k];
+    zero_rows<T, VEC>(z + k, v[k] < a.rows && !found, a.D, dW);
   }
 }
 
@@ -438,13 +473,11 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void emb_sum_kernel(SumArgs a, const T *__restrict__ g, T *__restrict__ dW) {
   __shared__ int32_t s_key[kMaxEntries + 2], s_pos[kMaxEntries];
   if ((int32_t)blockIdx.x >= a.blocks) {
-    const int32_t z = (int32_t)blockIdx.x - a.blocks, v = z * kZeroRows + (int32_t)threadIdx.x;
-    bool absent = false;
-    if (v < a.rows) {
-      const int32_t at = lower_bound(a.keys, a.n, v);
-      absent = !(at < a.n && a.keys[at] == v);
-    }
-    zero_rows<T, VEC>(z, absent, a.D, dW);
+    const int32_t z = (int32_t)blockIdx.x - a.blocks;
+    if (a.zero_steps == 1)
+      zero_absent<T, VEC, 1>(a, z, dW);
+    else
+      zero_absent<T, VEC, kZeroSteps>(a, z * kZeroSteps, dW);
     return;
   }
   const int per_block = a.G * a.per_group;
@@ -687,7 +720,7 @@ int check_common(int32_t dtype, int32_t id_bytes, int64_t n, int32_t rows, int32
   RK_CHECK_ARG(dtype == RK_F32 || dtype == RK_BF16 || dtype == RK_F16, "unknown element type %d", dtype);
   RK_CHECK_ARG(id_bytes == 4 || id_bytes == 8, "ids are int32 or int64, not of %d bytes", id_bytes);
   RK_CHECK_ARG(n >= 0 && rows >= 0 && D >= 1, "bad size: %lld ids, table %d x %d", (long long)n, rows, D);
-  RK_CHECK_ARG(n < (1ll << 31) - (1 << 24) && rows < INT32_MAX - 1, "more than 2^31 ids or rows");
+  RK_CHECK_ARG(n < (1ll << 31) - (1 << 24) && rows < (1ll << 31) - (1 << 24), "more than 2^31 ids or rows");
   return RK_OK;
 }
 
@@ -755,7 +788,7 @@ int launch_few(const SumArgs &a, const ID *ids, int64_t padding, const void *g, 
 
 template <typename T, int VEC>
 int launch_sum(const SumArgs &a, const void *g, void *dW, hipStream_t st) {
-  const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows);
+  const int64_t blocks = (int64_t)a.blocks + rk::ceil_div(a.rows, kZeroRows * a.zero_steps);
   RK_CHECK_ARG(blocks < rk::kMaxBlocks256, "too many ids for one call");
   emb_sum_kernel<T, VEC><<<(uint32_t)blocks, 256, 0, st>>>(a, (const T *)g, (T *)dW);
   RK_CHECK_LAUNCH("emb_sum_kernel");
@@ -803,7 +836,7 @@ int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t i
   int32_t *w = (int32_t *)ws;
   const Layout y = layout_of(n, rows, D, dtype);
   if (n > 0 && n <= kFewIds && rows < kFewRows - 1) {
-    const SumArgs a = {nullptr, nullptr, (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks, scale, (float *)w};
+    const SumArgs a = {nullptr, nullptr, (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks, 1, scale, (float *)w};
 #define RK_FEW(T, VEC)                                                          \
   (id_bytes == 8 ? launch_few<T, VEC>(a, (const int64_t *)ids, padding_idx, grad, d_weight, st) \
                  : launch_few<T, VEC>(a, (const int32_t *)ids, padding_idx, grad, d_weight, st))
@@ -817,8 +850,8 @@ int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t i
                                  : launch_sort((const int32_t *)ids, (int32_t)n, rows, padding_idx, y, w, st);
     if (rc) return rc;
   }
-  const SumArgs a = {w + y.keys[0], w + y.perm[0], (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks, scale,
-                     (float *)(w + y.pieces)};
+  const SumArgs a = {w + y.keys[0], w + y.perm[0], (int32_t)n, rows, D, y.L, y.G, y.per_group, y.blocks,
+                     rows < kManyRows ? 1 : kZeroSteps, scale, (float *)(w + y.pieces)};
   if (dtype == RK_F32) return D >= 4 ? launch_sum<float, 4>(a, grad, d_weight, st) : launch_sum<float, 1>(a, grad, d_weight, st);
   if (dtype == RK_BF16) return D >= 8 ? launch_sum<__bf16, 8>(a, grad, d_weight, st) : launch_sum<__bf16, 1>(a, grad, d_weight, st);
   return D >= 8 ? launch_sum<_Float16, 8>(a, grad, d_weight, st) : launch_sum<_Float16, 1>(a, grad, d_weight, st);

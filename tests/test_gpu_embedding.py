@@ -71,7 +71,8 @@ CASES = [
     (400, 100, 6000, "runs"), (500, 33, 20000, "same"), (26495, 128, 3200, "skewed"), (300, 256, 9000, "skewed"),
     (70000, 16, 50000, "skewed"), (300000, 10, 30000, "uniform"), (200, 2056, 700, "skewed"), (2, 1030, 5000, "uniform"),
     (511, 65, 10000, "uniform"), (40, 64, 512, "same"), (40, 64, 511, "runs"), (7050, 33, 513, "skewed"), (3, 300, 400, "uniform"), (9000000, 3, 300, "uniform"), (512, 64, 100000, "runs"), (4, 64, 200000, "uniform"),
-    (40, 1025, 9000, "runs"), (3, 1029, 4000, "same"),
+    (40, 1025, 9000, "runs"), (3, 1029, 4000, "same"), (2500001, 2, 9000, "uniform"),
+    (2100000, 5, 700, "skewed"),
 ]
 
 

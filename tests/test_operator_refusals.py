@@ -106,7 +106,7 @@ def test_c_abi_refuses_bad_embedding_calls():
     fwd = lambda dtype=0, bytes_=8, n=2, rows=4, D=4, ld=4, w=b, ids=b: (w, ld, rows, D, dtype, ids, bytes_, n, 1.0, b, None)  # noqa: E731,E501
     for kw, error in (({"dtype": 3}, "element type"), ({"bytes_": 2}, "int32 or int64"), ({"n": -1}, "bad size"),
                       ({"D": 0}, "bad size"), ({"rows": -1}, "bad size"), ({"ld": 3}, "overlap"), ({"w": None}, "null"),
-                      ({"ids": None}, "null"), ({"n": 1 << 31}, "2^31")):
+                      ({"ids": None}, "null"), ({"n": 1 << 31}, "2^31"), ({"rows": (1 << 31) - 100}, "2^31")):
         refused("rk_embedding_fwd", *fwd(**kw), error=error)
     assert _ffi.load().rk_embedding_fwd(*fwd(n=0)) == _ffi.RK_OK
     need = _ffi.load().rk_embedding_bwd_ws_bytes(2, 4, 4, 0)
