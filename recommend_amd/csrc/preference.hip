@@ -25,6 +25,7 @@ constexpr int kFewRows = 4096;       // rows that one workgroup joins
 // Pairs that one workgroup adds up behind more rows than that; more take two launches (4096 pairs 7.2 us, in two
 // launches 2.9 + 1.8 and a gap; 100000 pairs 129 us, 4.9 + 4.7).
 constexpr int kOnePairs = 4096;
+constexpr int kLongList = 512;       // places of a list that a wavefront adds up
 
 // A row's part is read by a workgroup, or by a wavefront (four parts in a workgroup): a row of 1000 scores
 // keeps 125 of 256 threads busy once.
@@ -154,12 +155,15 @@ __device__ __forceinline__ float row_logp(const Rows &a, int64_t row, const floa
 }
 
 // The lists' log-probabilities and the numbers of their places in use.  `lanes` threads for a list: a power of two up
-// to 64 (200000 lists of one place: 5.1 us, by a wavefront each 51).
-__global__ __launch_bounds__(kThreads) void lists_kernel(Rows a, const float2 *__restrict__ part,
-                                                         const float *__restrict__ score, float2 *__restrict__ stat,
-                                                         int average, int lanes, float *__restrict__ logps,
-                                                         int32_t *__restrict__ used) {
-  const int64_t s = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
+// to 64 (200000 lists of one place: 5.1 us, by a wavefront each 51), or 1024 where a list is long (LONG; two lists
+// of 100000 places: 104 us, by a wavefront each 1340; eight of 600: 4.0 and 10.7).
+template <bool LONG>
+__global__ __launch_bounds__(LONG ? kPairThreads : kThreads) void lists_kernel(Rows a, const float2 *__restrict__ part,
+                                                                              const float *__restrict__ score,
+                                                                              float2 *__restrict__ stat, int average, int lanes,
+                                                                              float *__restrict__ logps,
+                                                                              int32_t *__restrict__ used) {
+  const int64_t s = LONG ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
   const int lane = (int)threadIdx.x & (lanes - 1);
   if (s >= a.S) return;
   double sum = 0.0;
@@ -169,9 +173,23 @@ __global__ __launch_bounds__(kThreads) void lists_kernel(Rows a, const float2 *_
     sum += (double)row_logp(a, s * a.T + t, part, score, stat);
     ++n;
   }
-  for (int off = lanes / 2; off > 0; off >>= 1) {
+  for (int off = min(lanes, rk::kWave) / 2; off > 0; off >>= 1) {
     sum += __shfl_xor(sum, off, rk::kWave);
     n += __shfl_xor(n, off, rk::kWave);
+  }
+  if constexpr (LONG) {
+    __shared__ double s_sum[kPairThreads / rk::kWave];
+    __shared__ int32_t s_n[kPairThreads / rk::kWave];
+    if (threadIdx.x % rk::kWave == 0) {
+      s_sum[threadIdx.x / rk::kWave] = sum;
+      s_n[threadIdx.x / rk::kWave] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0)
+      for (int w = 1; w < kPairThreads / rk::kWave; ++w) {
+        sum += s_sum[w];
+        n += s_n[w];
+      }
   }
   if (lane == 0) {
     logps[s] = (float)(average && n > 0 ? sum / n : sum);
@@ -206,12 +224,13 @@ __device__ __forceinline__ float pair_term(float d, float beta, float eps, int k
 }
 
 // One workgroup: the pairs' terms, their slopes and the mean, added in a fixed order.  K > 0: it also forms the
-// lists' log-probabilities, from up to K rows for each thread (one launch instead of two).
+// lists' log-probabilities, from up to K rows for each thread (one launch instead of two), or a row for each `lanes`
+// threads, a power of two (two rows of 10^8 scores, 4096 parts each: 15 us where a thread for each took 494).
 template <int K>
 __global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float2 *__restrict__ part,
                                                              const float *__restrict__ score, float2 *__restrict__ stat,
                                                              const float *__restrict__ ref, int average, float beta,
-                                                             float eps, int kind, float *__restrict__ logps,
+                                                             float eps, int kind, int lanes, float *__restrict__ logps,
                                                              int32_t *__restrict__ used, float *__restrict__ slope_out,
                                                              float *__restrict__ loss) {
   constexpr bool ROWS = K > 0;
@@ -220,53 +239,65 @@ __global__ __launch_bounds__(kPairThreads) void pairs_kernel(Rows a, const float
   const int32_t P = a.S / 2;
   if constexpr (ROWS) {
     const int32_t rows = a.S * a.T;
+    const int32_t sub = (int32_t)threadIdx.x & (lanes - 1);
     bool in[K];                                            // (the loads of a thread's rows are in flight together)
+    int32_t at[K];
     float m[K], q[K], sc[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int32_t row = min(k * kPairThreads + (int32_t)threadIdx.x, rows - 1), s = row / a.T, t = row - s * a.T;
-      in[k] = k * kPairThreads + (int32_t)threadIdx.x < rows && a.items[s * a.ld_items + t] != a.ignore;
+      at[k] = (k * kPairThreads + (int32_t)threadIdx.x) / lanes;
+      const int32_t row = min(at[k], rows - 1), s = row / a.T, t = row - s * a.T;
+      in[k] = at[k] < rows && a.items[s * a.ld_items + t] != a.ignore;
       sc[k] = score[row];                                  // (not written for a place that is not in use, and not used)
       m[k] = -__FLT_MAX__;
       q[k] = 0.0f;
     }
-    for (int p = 0; p < a.parts; ++p) {
-      float2 o[K];
+    constexpr int U = K == 1 ? 8 : 1;                      // parts of a thread in flight
+    for (int p = sub; p < a.parts; p += U * lanes) {
+      float2 o[U][K];
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        o[k] = part[(int64_t)min(k * kPairThreads + (int32_t)threadIdx.x, rows - 1) * a.parts + p];
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int k = 0; k < K; ++k) merge(m[k], q[k], o[k].x, o[k].y);
+        for (int k = 0; k < K; ++k)
+          o[u][k] = part[(int64_t)min(at[k], rows - 1) * a.parts + min(p + u * lanes, a.parts - 1)];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (p + u * lanes < a.parts) merge(m[k], q[k], o[u][k].x, o[u][k].y);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int32_t row = k * kPairThreads + (int32_t)threadIdx.x;
-      if (row >= rows) break;
+      for (int off = lanes / 2; off > 0; off >>= 1) {
+        const float om = __shfl_xor(m[k], off, rk::kWave), os = __shfl_xor(q[k], off, rk::kWave);
+        merge(m[k], q[k], om, os);
+      }
+      const int32_t row = at[k];
+      if (row >= rows || sub != 0) continue;
       const float lq = logf(q[k]);
       if (in[k]) stat[row] = make_float2(m[k], lq);
       // a place that is not in use is marked by the one value that no log-probability has
       s_row[row] = in[k] ? (sc[k] - m[k]) - lq : __builtin_inff();
     }
     __syncthreads();
-    // 16 lanes for every list
-    const int sub = threadIdx.x % 16;
-    for (int32_t s0 = 0; s0 < a.S; s0 += kPairThreads / 16) {
-      const int32_t s = s0 + (int32_t)threadIdx.x / 16;
+    // up to 16 lanes for every list
+    const int per_list = a.T >= 16 ? 16 : a.T > 4 ? 8 : a.T > 1 ? 4 : 1, place = threadIdx.x & (per_list - 1);
+    for (int32_t s0 = 0; s0 < a.S; s0 += kPairThreads / per_list) {
+      const int32_t s = s0 + (int32_t)threadIdx.x / per_list;
       double sum = 0.0;
       int32_t n = 0;
       if (s < a.S)
-        for (int32_t t = sub; t < a.T; t += 16) {
+        for (int32_t t = place; t < a.T; t += per_list) {
           const float v = s_row[s * a.T + t];
           if (v == __builtin_inff()) continue;
           sum += (double)v;
           ++n;
         }
-#pragma unroll
-      for (int off = 8; off > 0; off >>= 1) {
-        sum += __shfl_xor(sum, off, 16);
-        n += __shfl_xor(n, off, 16);
+      for (int off = per_list / 2; off > 0; off >>= 1) {
+        sum += __shfl_xor(sum, off, rk::kWave);
+        n += __shfl_xor(n, off, rk::kWave);
       }
-      if (s < a.S && sub == 0) {
+      if (s < a.S && place == 0) {
         const float v = (float)(average && n > 0 ? sum / n : sum);
         s_logp[s] = logps[s] = v;
         used[s] = n;
@@ -473,11 +504,18 @@ int launch_rows_fwd(const Rows &a, const void *x, float *ws, const Ws &w, hipStr
 
 int launch_lists(const Rows &a, int average, float *stat, float *logps, int32_t *used, const float *ws, const Ws &w,
                  hipStream_t st) {
+  if (a.T > kLongList) {
+    RK_CHECK_ARG(4 * (int64_t)a.S < rk::kMaxBlocks256, "too many lists for one call");
+    lists_kernel<true><<<(uint32_t)a.S, kPairThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score, (float2 *)stat,
+                                                             average, kPairThreads, logps, used);
+    RK_CHECK_LAUNCH("lists_kernel");
+    return RK_OK;
+  }
   int lanes = 1;
   while (lanes < rk::kWave && lanes < a.T) lanes *= 2;
   const int64_t blocks = rk::ceil_div((int64_t)a.S, kThreads / lanes);
   RK_CHECK_ARG(blocks < rk::kMaxBlocks256, "too many lists for one call");
-  lists_kernel<<<(uint32_t)blocks, kThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score, (float2 *)stat, average,
+  lists_kernel<false><<<(uint32_t)blocks, kThreads, 0, st>>>(a, (const float2 *)(ws + w.part), ws + w.score, (float2 *)stat, average,
                                                     lanes, logps, used);
   RK_CHECK_LAUNCH("lists_kernel");
   return RK_OK;
@@ -499,9 +537,11 @@ int run_pairs(const Rows &a, const void *x, const float *ref, int average, float
   const float2 *part = (const float2 *)(ws + w.part);
   const int64_t rows = (int64_t)a.S * a.T;
 #define RK_PAIRS(K)                                                                                                    \
-  pairs_kernel<K><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind, logps, \
-                                              used, slope, loss)
+  pairs_kernel<K><<<1, kPairThreads, 0, st>>>(a, part, ws + w.score, (float2 *)stat, ref, average, beta, eps, kind, lanes, \
+                                              logps, used, slope, loss)
+  int lanes = 1;
   if (rows <= kPairThreads) {
+    while (lanes < rk::kWave && lanes < a.parts && 2 * lanes * rows <= kPairThreads) lanes *= 2;
     RK_PAIRS(1);
   } else if (rows <= kFewRows) {
     RK_PAIRS(kFewRows / kPairThreads);

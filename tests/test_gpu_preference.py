@@ -129,7 +129,9 @@ def test_preference_loss_vs_float64(kind, eps, S, T, V, dtype):
 @pytest.mark.parametrize("kind,eps", [("sigmoid", 0.1), ("squared", 0.0)])
 @pytest.mark.parametrize("S,T,V,dtype", [(8192, 1, 5, torch.float32), (8194, 1, 5, torch.float16), (10002, 1, 41, torch.float32),
                                          (16500, 3, 18, torch.bfloat16), (1000, 5, 30, torch.float32),
-                                         (66, 70, 33, torch.float32)])
+                                         (66, 70, 33, torch.float32), (4, 1500, 20, torch.float32),
+                                         (10, 513, 9, torch.bfloat16), (2, 1, 70001, torch.bfloat16),
+                                         (130, 1, 40000, torch.float32), (260, 4, 9001, torch.float32)])
 def test_many_lists_vs_float64(kind, eps, S, T, V, dtype):
     test_preference_loss_vs_float64(kind, eps, S, T, V, dtype)
 
