@@ -327,8 +327,8 @@ int rk_adam_update_f32(const rk_adam_tensor *tensors_host, int32_t n_tensors, in
 /* The nn.Embedding lookups of the reference's models (model/Main_Model.py:79,98) with a factor:
  * out[i, :] = scale * weight[ids[i], :] (product in fp32, rounded once to the table's type).
  * weight: rows x D of element type dtype (RK_F32 / RK_BF16 / RK_F16), ld_weight elements between
- * rows; any D >= 1 and any alignment of whole elements.  ids: n int32 (id_bytes 4) or int64 (8).
- * An id outside [0, rows) reads nothing and gives a row of NaN. */
+ * rows; any D >= 1 below 2^31 - 2^24 and any alignment of whole elements.  ids: n int32 (id_bytes 4)
+ * or int64 (8).  An id outside [0, rows) reads nothing and gives a row of NaN. */
 int rk_embedding_fwd(const void *weight, int64_t ld_weight, int32_t rows, int32_t D, int32_t dtype,
                      const void *ids, int32_t id_bytes, int64_t n, float scale, void *out, void *stream);
 /* d_weight[v, :] = scale * sum over { i : ids[i] = v } of grad[i, :], every row of d_weight written

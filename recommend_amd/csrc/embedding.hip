@@ -309,7 +309,9 @@ __device__ __forceinline__ int32_t lower_bound(const int32_t *__restrict__ keys,
   return lo;
 }
 
-// zeros in row z * kZeroRows + threadIdx.x where `absent` says so, a wavefront's 64 rows together
+// Zeros in row z * kZeroRows + threadIdx.x where `absent` says so, a wavefront's 64 rows together.  A lane carries row
+// and column of its next vector along: the number of the 64 rows' vectors, which rows of 2^25 vectors take past 32 bits,
+// is never formed.
 template <typename T, int VEC>
 __device__ __forceinline__ void zero_rows(int32_t z, bool absent, int32_t D, T *__restrict__ dW) {
   const uint64_t mask = __ballot(absent);
@@ -319,9 +321,16 @@ __device__ __forceinline__ void zero_rows(int32_t z, bool absent, int32_t D, T *
   rk::Pack<T, VEC> zero;
 #pragma unroll
   for (int i = 0; i < rk::Pack<T, VEC>::kWords; ++i) zero.w[i] = 0u;
-  for (int i = lane; i < rk::kWave * per_row; i += rk::kWave) {
-    const int r = i / per_row;
-    if ((mask >> r) & 1) zero.store(dW + (row0 + r) * D + min((i - r * per_row) * VEC, D - VEC));
+  const int step_r = rk::kWave / per_row, step_c = rk::kWave - step_r * per_row;   // (a column step is less than a row)
+  int r = lane / per_row, c = lane - r * per_row;
+  while (r < rk::kWave) {
+    if ((mask >> r) & 1) zero.store(dW + (row0 + r) * D + min(c * VEC, D - VEC));
+    r += step_r;
+    c += step_c;
+    if (c >= per_row) {
+      c -= per_row;
+      ++r;
+    }
   }
 }
 
@@ -721,6 +730,8 @@ int check_common(int32_t dtype, int32_t id_bytes, int64_t n, int32_t rows, int32
   RK_CHECK_ARG(id_bytes == 4 || id_bytes == 8, "ids are int32 or int64, not of %d bytes", id_bytes);
   RK_CHECK_ARG(n >= 0 && rows >= 0 && D >= 1, "bad size: %lld ids, table %d x %d", (long long)n, rows, D);
   RK_CHECK_ARG(n < (1ll << 31) - (1 << 24) && rows < (1ll << 31) - (1 << 24), "more than 2^31 ids or rows");
+  // (a lane's next column is formed before it is compared with the width)
+  RK_CHECK_ARG(D < (1ll << 31) - (1 << 24), "more than 2^31 columns");
   return RK_OK;
 }
 
