@@ -335,18 +335,13 @@ class FusedAdamW(torch.optim.Optimizer):
                     st["step"] = torch.tensor(t)
         return super().state_dict()
 
-    def load_state_dict(self, state_dict):
-        """Moments and step count of a checkpoint: this optimizer's with either number of bits, or
-        torch.optim.AdamW's.  Moments are converted to the form this optimizer holds.  Buffers that exist
-        keep their memory and take the checkpoint's values, so a step recorded in a HIP graph before the
-        load goes on with them.  Call it outside graph capture."""
-        old = {p: dict(st) for p, st in self.state.items()}
-        saved = state_dict["state"]
-        order = [i for g in state_dict["param_groups"] for i in g["params"]]
-        super().load_state_dict(state_dict)
-        # (torch casts floating state to the parameter's type on the way: the values are taken from the
-        # checkpoint itself)
-        for i, p in zip(order, [p for g in self.param_groups for p in g["params"]]):
+    def _moments_of(self, state_dict):
+        """{parameter: its state} of a checkpoint, in the form this optimizer holds it."""
+        saved, groups = state_dict["state"], state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return {}                                # (another model's: torch says so)
+        fresh = {}
+        for i, p in zip([i for g in groups for i in g["params"]], [p for g in self.param_groups for p in g["params"]]):
             src = saved.get(i)
             if not src or not ("exp_avg" in src or "exp_avg8" in src):
                 continue
@@ -362,12 +357,36 @@ class FusedAdamW(torch.optim.Optimizer):
             else:
                 st["exp_avg"] = decode_moment(src["exp_avg8"], src["exp_avg8_scale"], p)
                 st["exp_avg_sq"] = decode_moment(src["exp_avg_sq8"], src["exp_avg_sq8_scale"], p).square()
+            fresh[p] = st
+        return fresh
+
+    def load_state_dict(self, state_dict):
+        """Moments and step count of a checkpoint: this optimizer's with either number of bits, or
+        torch.optim.AdamW's.  Moments are converted to the form this optimizer holds.  Buffers that exist
+        keep their memory and take the checkpoint's values (zeros, where it has no moments of their parameter:
+        one saved before the first step has none), so a step recorded in a HIP graph before the load goes on
+        with them.  Buffers of another form than the checkpoint's become are not used again, and not freed
+        either.  Call it outside graph capture."""
+        old = {p: {k: v for k, v in st.items() if k != "step" and torch.is_tensor(v)} for p, st in self.state.items()}
+        # (torch casts floating state to the parameter's type on the way: the values are taken from the checkpoint
+        # itself, and before anything is replaced, so that a checkpoint of other sizes leaves all as it was)
+        fresh = self._moments_of(state_dict)
+        super().load_state_dict(state_dict)
+        for p, st in fresh.items():
+            held = old.pop(p, {})
             for k, v in st.items():
-                have = old.get(p, {}).get(k)
-                if k != "step" and have is not None and have.shape == v.shape and have.dtype == v.dtype:
+                have = held.get(k)
+                if have is not None and have.shape == v.shape and have.dtype == v.dtype:
                     have.copy_(v)
-                    st[k] = have
+                    st[k] = held.pop(k)
+            self._held += held.values()
             self.state[p] = st
+        for p, held in old.items():
+            if not held:
+                continue
+            for v in held.values():
+                (v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v).zero_()
+            self.state[p] = held
         self._restored_step = max((int(st["step"]) for st in self.state.values() if "step" in st), default=0)
         if self._dev is not None:
             self.step_count.fill_(self._restored_step)

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from recommend_amd import ops
+from recommend_amd.optim import FusedAdamW
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -28,3 +29,44 @@ def test_rows_whose_vectors_pass_32_bits(dtype, D, n):
     dw, = torch.autograd.grad(out, table, grad)
     assert bool((dw[0] == 0).all()) and bool((dw[2] == 0).all())
     assert torch.equal(dw[1], 2 * grad[0] if n else torch.zeros_like(dw[1]))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_recorded_step_goes_on_after_a_checkpoint_without_its_moments(bits):
+    """A step is recorded, then the checkpoint from before the first step is loaded: replays do what a new optimizer
+    does, and touch nothing that was allocated since."""
+    g = torch.Generator().manual_seed(5)
+    start = [torch.randn(s, generator=g).to(DEV) for s in ((100, 64), (64,))]
+    ours = [torch.nn.Parameter(w.clone()) for w in start]
+    opt = FusedAdamW(ours, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+    saved = opt.state_dict()
+    for p in ours:
+        p.grad = torch.randn(p.shape, generator=g).to(DEV)
+    for _ in range(2):
+        opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    graph.replay()
+    opt.load_state_dict(saved)
+    with torch.no_grad():
+        for p, w in zip(ours, start):
+            p.copy_(w)
+    # every size that a moment has had: freed ones would be given out here
+    others = [torch.full((n,), 7, dtype=torch.uint8, device=DEV) for n in (6400, 25600, 400, 256) for _ in range(20)]
+    fresh = [torch.nn.Parameter(w.clone()) for w in start]
+    same = FusedAdamW(fresh, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+    for k in range(4):
+        for p, q in zip(ours, fresh):
+            p.grad.copy_(torch.randn(p.shape, generator=g))
+            q.grad = p.grad.clone()
+        if k < 3:
+            graph.replay()
+        else:
+            opt.step()
+        same.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ours, fresh)) and int(opt.step_count) == int(same.step_count) == k + 1
+    assert all(bool((o == 7).all()) for o in others)
+    for p, q in zip(ours, fresh):
+        assert all(torch.equal(v.view(torch.uint8), same.state[q][k].view(torch.uint8)) for k, v in opt.state[p].items())

@@ -1,0 +1,80 @@
+"""What FusedAdamW's load_state_dict does to the moments that exist, on the host: a step recorded in a HIP graph holds
+their addresses, so no load may free them."""
+import pytest
+import torch
+
+from recommend_amd.optim import FusedAdamW, encode_moment
+
+
+def optimizer(bits, shapes=((100, 64), (64,), ())):
+    """With moments as a step makes them (steps need a GPU)."""
+    g = torch.Generator().manual_seed(1)
+    params = [torch.nn.Parameter(torch.randn(s, generator=g)) for s in shapes]
+    opt = FusedAdamW(params, state_bits=bits)
+    for p in params:
+        m, v = torch.randn(p.shape, generator=g), torch.rand(p.shape, generator=g)
+        if opt._is8(p):
+            st = dict(zip(("exp_avg8", "exp_avg8_scale"), encode_moment(m)))
+            st.update(zip(("exp_avg_sq8", "exp_avg_sq8_scale"), encode_moment(v, True)))
+        else:
+            st = {"exp_avg": m, "exp_avg_sq": v}
+        opt.state[p].update(st, step=torch.tensor(3.0))
+    return opt, params
+
+
+def addresses(opt, p):
+    return {k: v.data_ptr() for k, v in opt.state[p].items() if k != "step"}
+
+
+def cleared(opt, p):
+    return all(bool((v.float() == 0).all()) for k, v in opt.state[p].items() if k != "step")
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_checkpoint_from_before_the_first_step_clears_in_place(bits):
+    opt, params = optimizer(bits)
+    first = FusedAdamW([torch.nn.Parameter(p.detach().clone()) for p in params], state_bits=bits).state_dict()
+    assert not first["state"]
+    held = [addresses(opt, p) for p in params]
+    opt.load_state_dict(first)
+    assert [addresses(opt, p) for p in params] == held and all(held)
+    assert all(cleared(opt, p) for p in params) and opt._restored_step == 0
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_checkpoint_without_one_parameter_clears_that_one(bits):
+    opt, params = optimizer(bits)
+    saved = optimizer(bits)[0].state_dict()
+    want = {k: v.clone() for k, v in saved["state"][1].items()}
+    saved["state"][0] = {"momentum_buffer": torch.ones(100, 64)}          # another optimizer's
+    del saved["state"][2]
+    held = [addresses(opt, p) for p in params]
+    opt.load_state_dict(saved)
+    assert [addresses(opt, p) for p in params] == held
+    assert cleared(opt, params[0]) and cleared(opt, params[2]) and "momentum_buffer" not in opt.state[params[0]]
+    assert all(torch.equal(opt.state[params[1]][k], v) for k, v in want.items())
+    assert opt._restored_step == 3
+
+
+def test_buffers_that_cannot_be_used_again_are_not_freed():
+    """Moments of another form than the checkpoint's become (the threshold was moved): a recorded step still has them."""
+    opt, params = optimizer(8)
+    saved = optimizer(8)[0].state_dict()
+    old = {v.data_ptr() for k, v in opt.state[params[0]].items() if k != "step"}
+    opt.min_8bit_size = 1 << 20
+    opt.load_state_dict(saved)
+    assert set(opt.state[params[0]]) == {"step", "exp_avg", "exp_avg_sq"}
+    assert old <= {t.data_ptr() for t in opt._held}
+
+
+def test_a_checkpoint_of_other_sizes_leaves_everything_as_it_was():
+    opt, params = optimizer(32)
+    held = [addresses(opt, p) for p in params]
+    values = [v.clone() for p in params for v in opt.state[p].values()]
+    other = optimizer(32, ((100, 64), (63,), ()))[0].state_dict()
+    with pytest.raises(RuntimeError):
+        opt.load_state_dict(other)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(optimizer(32, ((100, 64),))[0].state_dict())
+    assert [addresses(opt, p) for p in params] == held
+    assert all(torch.equal(a, b) for a, b in zip([v for p in params for v in opt.state[p].values()], values))
