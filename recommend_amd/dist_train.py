@@ -28,6 +28,7 @@ from . import fused
 from .dist import (HipRowBlock, RowShardedGraph, _rows_csr, all_gather_rows_into, all_reduce_tensor,
                    node_range, reduce_scatter_rows)
 from .model import TEST, TESTModel, _ItemProjection
+from .train_step import UNSAID, clip_norm
 
 
 class _HipNormalizer:
@@ -285,15 +286,16 @@ class ShardedTrainStep:
     With an optimizer that clips inside its update (recommend_amd.optim.FusedClipAdam) the step has
     no per-parameter launches after the backward pass: one flat all-reduce whose slices BECOME the
     gradients, then the optimizer's two launches.  `graphed()` records the step, collectives
-    included, as one HIP graph."""
+    included, as one HIP graph.  max_grad_norm as in train_step.GraphedTrainStep."""
 
     PER_SAMPLE_KEYS = ("user_ids", "item_ids", "neg_items", "neg_rank", "ratings")
 
     def __init__(self, model: ShardedTESTModel, optimizer: torch.optim.Optimizer,
-                 loss_fn: Callable[[Dict, Dict], torch.Tensor], max_grad_norm: Optional[float] = 1.0,
+                 loss_fn: Callable[[Dict, Dict], torch.Tensor], max_grad_norm: Optional[float] = UNSAID,
                  sharded_params: Optional[List[torch.Tensor]] = None, per_sample_keys=None):
         self.model, self.opt, self.loss_fn = model, optimizer, loss_fn
-        self.max_grad_norm = max_grad_norm
+        # an optimizer that clips inside its own update sums the shards' norms over the ranks itself
+        self.max_grad_norm, self._opt_clips = clip_norm(optimizer, max_grad_norm)
         self.group, self.world, self.rank = model.group, model.world, model.rank
         self.per_sample_keys = tuple(per_sample_keys or self.PER_SAMPLE_KEYS)
         # as clip_grad_norm_(model.parameters()) and the optimizer see them (train/graph_trainer.py:151-156)
@@ -305,12 +307,8 @@ class ShardedTrainStep:
         self.replicated = [p for p in self.params if id(p) not in sh]
         self._synced = None      # the replicated parameters some rank has a gradient for
         self.last_grad_norm = None
-        # an optimizer that clips inside its own update and sums the shards' norms over the ranks itself
-        self._opt_clips = hasattr(optimizer, "max_grad_norm")
-        if self._opt_clips:
-            optimizer.max_grad_norm = max_grad_norm
-            if self.sharded and not getattr(optimizer, "_sharded", None):
-                raise ValueError("build the optimizer with sharded_params=... and group=... for row-sharded parameters")
+        if self._opt_clips and self.sharded and not getattr(optimizer, "_sharded", None):
+            raise ValueError("build the optimizer with sharded_params=... and group=... for row-sharded parameters")
 
     def split(self, batch):
         """This rank's samples of the global batch: the per-sample entries (`per_sample_keys`) are

@@ -17,6 +17,21 @@ import torch
 
 from . import ops
 
+UNSAID = object()       # a clipping norm that the caller leaves to the optimizer
+
+
+def clip_norm(optimizer, max_grad_norm):
+    """(norm that a training step clips its gradients to, whether the optimizer does it inside its own update).
+    A norm that the caller gives, None among them, goes to such an optimizer; where none is given its own
+    stays, and without one it is the reference trainer's 1.0 (train/graph_trainer.py:151-156)."""
+    inside = hasattr(optimizer, "max_grad_norm")
+    if max_grad_norm is UNSAID:
+        own = getattr(optimizer, "max_grad_norm", None)
+        max_grad_norm = 1.0 if own is None else own
+    if inside:
+        optimizer.max_grad_norm = max_grad_norm
+    return max_grad_norm, inside
+
 
 class GraphedStep:
     """body(batch) -> loss tensor: one whole training step (zero_grad excluded) on the current
@@ -85,18 +100,17 @@ class GraphedTrainStep(GraphedStep):
     def __init__(self, model: torch.nn.Module, optimizer: torch.optim.Optimizer,
                  loss_fn: Callable[[Dict, Dict], torch.Tensor], example_batch: Dict[str, torch.Tensor],
                  constants: Optional[Dict[str, torch.Tensor]] = None,
-                 max_grad_norm: Optional[float] = 1.0, warmup_steps: int = 3):
+                 max_grad_norm: Optional[float] = UNSAID, warmup_steps: int = 3):
         """example_batch: a batch dict as the loader yields it (device tensors); its tensors fix
         the captured shapes, and the warm-up steps train on it (they are real steps).  constants: entries every batch carries unchanged (e.g. the
         user->positives CSR for in-kernel negative lookup); they are not copied per step.
-        The optimizer must be capturable (recommend_amd.optim.FusedClipAdam, or e.g.
+        max_grad_norm (None: no clipping): where it is not given, that of an optimizer which clips inside its
+        update and was given one, otherwise 1.0.
+        The optimizer must be capturable (recommend_amd.optim.FusedClipAdam or FusedAdamW, or e.g.
         torch.optim.Adam(capturable=True))."""
         self.model, self.opt, self.loss_fn = model, optimizer, loss_fn
-        self.max_grad_norm = max_grad_norm
-        # an optimizer that clips inside its own update (recommend_amd.optim.FusedClipAdam)
-        self._opt_clips = hasattr(optimizer, "max_grad_norm")
-        if self._opt_clips:
-            optimizer.max_grad_norm = max_grad_norm
+        # (FusedClipAdam and FusedAdamW of recommend_amd.optim clip inside their own updates)
+        self.max_grad_norm, self._opt_clips = clip_norm(optimizer, max_grad_norm)
         self.params = [p for p in model.parameters() if p.requires_grad]
         super().__init__(self._train_body, lambda: self.opt.zero_grad(set_to_none=True), example_batch, constants,
                          warmup_steps)

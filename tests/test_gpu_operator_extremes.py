@@ -5,6 +5,7 @@ import torch
 
 from recommend_amd import ops
 from recommend_amd.optim import FusedAdamW
+from recommend_amd.train_step import GraphedTrainStep
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -70,3 +71,22 @@ def test_recorded_step_goes_on_after_a_checkpoint_without_its_moments(bits):
     assert all(bool((o == 7).all()) for o in others)
     for p, q in zip(ours, fresh):
         assert all(torch.equal(v.view(torch.uint8), same.state[q][k].view(torch.uint8)) for k, v in opt.state[p].items())
+
+
+def test_recorded_training_step_clips_to_the_norm_that_the_optimizer_was_given():
+    g = torch.Generator().manual_seed(6)
+    model = torch.nn.Linear(8, 1, bias=False).to(DEV)
+    batch = {"x": torch.randn(32, 8, generator=g).to(DEV)}
+    twin = torch.nn.Parameter(model.weight.detach().clone())
+    opt, same = FusedAdamW(model.parameters(), lr=0.1, max_grad_norm=0.25), FusedAdamW([twin], lr=0.1, max_grad_norm=0.25)
+    net = torch.nn.Module()
+    net.weight = model.weight
+    net.forward = lambda b: b["x"] * net.weight
+    step = GraphedTrainStep(net, opt, lambda out, b: 50 * out.square().mean(), batch, warmup_steps=1)
+    step(batch)
+    for _ in range(2):
+        twin.grad, = torch.autograd.grad(50 * (batch["x"] * twin).square().mean(), twin)
+        same.step()
+    torch.cuda.synchronize()
+    assert opt.max_grad_norm == 0.25 and float(opt.grad_norm) > 0.25
+    assert torch.equal(model.weight, twin) and torch.equal(opt.state[model.weight]["exp_avg"], same.state[twin]["exp_avg"])
