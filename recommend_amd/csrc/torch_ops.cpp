@@ -306,7 +306,7 @@ std::pair<Tensor, Tensor> lists(const char *what, const Tensor &scores_in, const
                                     items.data_ptr<int64_t>(), geo.T, ignore, average, stat, logps.data_ptr<float>(),
                                     (int32_t *)used, ws, ws_bytes, stream_of(scores.device())));
       } else {
-        const Tensor ref = ref_in.detach().to(at::kFloat).contiguous();
+        const Tensor ref = ref_in.to(at::kFloat).contiguous();
         loss = at::empty({}, f32);
         check(abi.rk_preference_fwd(scores.data_ptr(), geo.kind, geo.S, geo.T, geo.V, geo.stride_s, geo.stride_t,
                                     items.data_ptr<int64_t>(), geo.T, ignore, average, ref.data_ptr<float>(), (float)beta,
@@ -351,6 +351,9 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor &scores, const Tensor &it
   TORCH_CHECK_VALUE(ref.dim() == 1 && ref.size(0) == S, "preference_loss: one reference log-probability per list, got ",
                     ref.sizes(), " for ", S);
   TORCH_CHECK_VALUE(ref.is_floating_point(), "preference_loss: reference log-probabilities are floating point");
+  TORCH_CHECK_VALUE(!records(ref), "preference_loss: the reference log-probabilities get no gradient: detach them, or "
+                    "compute them under torch.no_grad()");
+  no_tangent("preference_loss (of ref_logps)", ref);
   if (scores.is_cuda()) need_same_device(scores, ref);
   return lists("preference_loss", scores, items, ref, ignore, average, beta, smoothing, kind);
 }

@@ -150,7 +150,8 @@ def preference_loss(scores, items, ref_logps, beta=0.1, label_smoothing=0.0, kin
 
     scores: [2P, T, V] catalogue scores, the P preferred lists first, then their P counterparts in the same
     order (or [2P, V] for lists of one item); items: [2P, T] the items at the lists' places, `ignore_index`
-    where a place is not in use; ref_logps: [2P] list_logps of the reference model.  With
+    where a place is not in use; ref_logps: [2P] list_logps of the reference model, constants: values that require
+    a gradient are refused.  With
     d = (logps - ref)[preferred] - (logps - ref)[other] the term of a pair is
       "sigmoid"  -(1 - label_smoothing) logsigmoid(beta d) - label_smoothing logsigmoid(-beta d)
       "hinge"    max(0, 1 - beta d)
