@@ -349,7 +349,8 @@ int rk_embedding_bwd(const void *grad, int32_t dtype, const void *ids, int32_t i
  *   logps[s] = sum_t (x[s, t, items[s, t]] - log sum_j exp x[s, t, j])   over the places in use
  * (average != 0: divided by their number; a list without any has 0).  Places that are not in use
  * are not read.  An item outside [0, V) makes its list's result NaN.  stat: [S * T][2] floats and
- * used: [S] int32, kept for the backward call.  ws: rk_list_logps_ws_bytes() bytes of scratch. */
+ * used: [S] int32, kept for the backward call.  ws: rk_list_logps_ws_bytes() bytes of scratch.  stat
+ * and ws are 8-byte aligned. */
 size_t rk_list_logps_ws_bytes(int32_t S, int32_t T, int32_t V);
 int rk_list_logps_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, int32_t V,
                       int64_t stride_s, int64_t stride_t, const int64_t *items, int64_t ld_items,

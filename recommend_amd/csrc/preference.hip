@@ -563,6 +563,9 @@ int run_pairs(const Rows &a, const void *x, const float *ref, int average, float
   return RK_OK;
 }
 
+// `stat` and the workspace hold pairs of floats and, behind many rows, doubles
+bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
 constexpr int64_t kStreamBytes = 64 << 20;   // gradients from this size on are stored past the caches
 
 template <typename T>
@@ -610,6 +613,7 @@ int rk_list_logps_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
   RK_CHECK_ARG(S == 0 || T > 0, "lists without places");
   if (S == 0) return RK_OK;
   RK_CHECK_ARG(scores && stat && logps && used && ws, "null pointer");
+  RK_CHECK_ARG(aligned8(stat) && aligned8(ws), "stat and workspace must be 8-byte aligned");
   RK_CHECK_ARG(ws_bytes >= rk_list_logps_ws_bytes(S, T, V), "workspace too small");
   return RK_BY_TYPE(run_lists, a, scores, average, stat, logps, used, (float *)ws, (hipStream_t)stream);
 }
@@ -626,6 +630,7 @@ int rk_preference_fwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
   RK_CHECK_ARG(label_smoothing >= 0.0f && label_smoothing <= 1.0f, "label smoothing outside [0, 1]");
   RK_CHECK_ARG(label_smoothing == 0.0f || kind == RK_PREF_SIGMOID, "label smoothing is part of the sigmoid form only");
   RK_CHECK_ARG(scores && ref_logps && stat && logps && used && slope && loss && ws, "null pointer");
+  RK_CHECK_ARG(aligned8(stat) && aligned8(ws), "stat and workspace must be 8-byte aligned");
   RK_CHECK_ARG(ws_bytes >= rk_list_logps_ws_bytes(S, T, V), "workspace too small");
   return RK_BY_TYPE(run_pairs, a, scores, ref_logps, average, beta, label_smoothing, kind, stat, logps, used, slope, loss,
                     (float *)ws, (hipStream_t)stream);
@@ -639,6 +644,7 @@ int rk_list_logps_bwd(const void *scores, int32_t dtype, int32_t S, int32_t T, i
   if (int rc = make_rows(a, dtype, S, T, V, stride_s, stride_t, items, ld_items, ignore_index, kWantBwd)) return rc;
   if (S == 0 || T == 0) return RK_OK;
   RK_CHECK_ARG(scores && stat && used && d_scores, "null pointer");
+  RK_CHECK_ARG(aligned8(stat), "stat must be 8-byte aligned");
   RK_CHECK_ARG(!g_loss || slope, "the gradient of the loss needs the slopes of rk_preference_fwd");
   return RK_BY_TYPE(run_bwd, a, scores, stat, g_loss, slope, g_logps, average, used, d_scores, (hipStream_t)stream);
 }

@@ -31,3 +31,14 @@ def test_reference_values_that_require_a_gradient_are_refused():
         preference_loss(scores, items, ref)
     with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="ref_logps"):
         preference_loss(scores, items, torch.autograd.forward_ad.make_dual(torch.zeros(2), torch.ones(2)))
+
+
+def test_list_calls_refuse_addresses_that_are_not_8_byte_aligned():
+    buf, lib = np.zeros(4096, np.float64), _ffi.load()
+    b, odd = _ffi.ptr(buf), buf.ctypes.data + 4
+    need = lib.rk_list_logps_ws_bytes(4, 3, 5)
+    geo = (b, 0, 4, 3, 5, 15, 5, b, 3, -100, 0)
+    for stat, ws in ((odd, b), (b, odd)):
+        refused("rk_list_logps_fwd", *geo, stat, b, b, ws, need, None, error="8-byte aligned")
+        refused("rk_preference_fwd", *geo, b, 0.1, 0.0, 0, stat, b, b, b, b, ws, need, None, error="8-byte aligned")
+    refused("rk_list_logps_bwd", *geo, odd, b, b, b, b, b, None, error="8-byte aligned")
