@@ -213,6 +213,19 @@ class FusedAdamW(torch.optim.Optimizer):
     torch.float8_e4m3fn codes with one fp32 scale per 64 consecutive elements (`exp_avg8`,
     `exp_avg8_scale`, `exp_avg_sq8`, `exp_avg_sq8_scale`): 2.1 bytes for each element instead of 8.
 
+    What 8-bit moments do not follow: codes are rounded to nearest after every step, so a root changes its code only
+    where one step moves it by half a code (3 to 6 %) against the largest of its block of 64.  With betas[1] = 0.999 a
+    step takes at most 0.05 % off a root: against its block it never falls, and rises only for gradients several
+    times as large.  Simulated, 4,000 steps, scales of a block's elements spread by e^1, against 32-bit moments:
+      steady gradients                          cosine of the update 0.988, roots (99.8 % of them) 0.67 to 1.70 times
+      all gradients a tenth from step 500 on    the same: a block's scale follows
+      every second element's a tenth            cosine 0.96, 0.88, 0.80 at step 1,000, 2,000, 4,000, the update's norm up to
+                                                1.96 times; their roots 5.7 times too large (median; their rate is too
+                                                small by that), their neighbours' down to 0.24 of what they should be
+      every second element's threefold          cosine 0.85; the others' roots 2.4 times too large, theirs down to 0.35
+    The third case with betas[1] = 0.99: 0.82, with 0.95: 0.996.  Where the scales of neighbouring elements come apart
+    during training take state_bits=32 (or a min_8bit_size that leaves those tensors out), or betas[1] up to 0.95.
+
     As with FusedClipAdam the step count and the learning rates live in device memory, a step can be
     recorded in a HIP graph after one eager step, and parameters without a gradient take no part.  The
     step count is one for all parameters.  Parameters must not share memory (one object given twice in a group
