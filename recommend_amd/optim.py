@@ -228,7 +228,10 @@ class FusedAdamW(torch.optim.Optimizer):
 
     As with FusedClipAdam the step count and the learning rates live in device memory, a step can be
     recorded in a HIP graph after one eager step, and parameters without a gradient take no part.  The
-    step count is one for all parameters.  Parameters must not share memory (one object given twice in a group
+    step count is one for all parameters, where torch.optim.AdamW counts each one's own: a parameter whose first
+    gradient comes late is corrected with the count of the others (with the default betas its first updates are up to
+    (1 - beta1) / (1 - beta2)^(1/2) = 3.2 times as large), and a checkpoint whose counts differ continues with the
+    largest.  Parameters must not share memory (one object given twice in a group
     is refused).  Checkpoints load across state_bits and from torch.optim.AdamW."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None,

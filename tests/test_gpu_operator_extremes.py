@@ -90,3 +90,18 @@ def test_recorded_training_step_clips_to_the_norm_that_the_optimizer_was_given()
     torch.cuda.synchronize()
     assert opt.max_grad_norm == 0.25 and float(opt.grad_norm) > 0.25
     assert torch.equal(model.weight, twin) and torch.equal(opt.state[model.weight]["exp_avg"], same.state[twin]["exp_avg"])
+
+
+def test_a_late_parameter_is_corrected_with_the_common_count():
+    """20 steps without it, then its first gradient: m = 0.1 g, v = 0.001 g^2, corrected with count 21.  The update rounds
+    a dozen times (16 u) and the parameter once."""
+    a, late = (torch.nn.Parameter(torch.ones(70, device=DEV)) for _ in range(2))
+    opt = FusedAdamW([a, late], lr=1e-2, weight_decay=0.0, eps=0.0)
+    for _ in range(20):
+        a.grad = torch.ones_like(a)
+        opt.step()
+    late.grad = torch.full_like(late, 3.0)
+    opt.step()
+    move = 1e-2 / (1 - 0.9 ** 21) * 0.1 / (0.001 / (1 - 0.999 ** 21)) ** 0.5
+    assert int(opt.step_count) == 21
+    assert float((late.detach().double() - (1 - move)).abs().max()) <= (16 * move + 1) * 2.0 ** -24

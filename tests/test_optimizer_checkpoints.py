@@ -78,3 +78,15 @@ def test_a_checkpoint_of_other_sizes_leaves_everything_as_it_was():
         opt.load_state_dict(optimizer(32, ((100, 64),))[0].state_dict())
     assert [addresses(opt, p) for p in params] == held
     assert all(torch.equal(a, b) for a, b in zip([v for p in params for v in opt.state[p].values()], values))
+
+
+def test_counts_that_differ_continue_with_the_largest():
+    w = [torch.nn.Parameter(torch.ones(3)) for _ in range(2)]
+    theirs = torch.optim.AdamW(w)
+    for k in range(4):
+        w[0].grad, w[1].grad = torch.ones(3), torch.ones(3) if k == 3 else None
+        theirs.step()
+    assert [int(theirs.state[p]["step"]) for p in w] == [4, 1]
+    opt = FusedAdamW([torch.nn.Parameter(torch.ones(3)) for _ in range(2)])
+    opt.load_state_dict(theirs.state_dict())
+    assert opt._restored_step == 4
