@@ -44,42 +44,59 @@ def torch_ops_command(out):
             "-ltorch_python"]
 
 
-def needs_build():
-    if not os.path.exists(LIB_PATH) or not os.path.exists(TORCH_OPS_PATH):
+def _stale(path, sources):
+    """Whether `path` is missing or older than one of `sources`, the header or this file."""
+    if not os.path.exists(path):
         return True
-    t = min(os.path.getmtime(LIB_PATH), os.path.getmtime(TORCH_OPS_PATH))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
-    deps.append(os.path.join(HERE, "..", "include", "recommend_amd.h"))
-    deps.append(os.path.abspath(__file__))
-    return any(os.path.getmtime(d) > t for d in deps)
+    deps = [os.path.join(CSRC, f) for f in sources] + [os.path.join(HERE, "..", "include", "recommend_amd.h"),
+                                                       os.path.abspath(__file__)]
+    return any(os.path.getmtime(d) > os.path.getmtime(path) for d in deps)
+
+
+def needs_library():
+    return _stale(LIB_PATH, [f for f in os.listdir(CSRC) if f != TORCH_OPS])
+
+
+def needs_torch_ops():
+    return _stale(TORCH_OPS_PATH, [TORCH_OPS])
+
+
+def needs_build():
+    return needs_library() or needs_torch_ops()
 
 
 def build(force=False, verbose=True):
-    if not force and not needs_build():
-        return LIB_PATH
+    """The library needs hipcc alone; it is complete where the torch module, compiled beside it, fails (which raises)."""
+    library, module = force or needs_library(), force or needs_torch_ops()
     os.makedirs(LIB_DIR, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    objs = []
-    procs = []
-    for src in SOURCES:
-        obj = os.path.join(LIB_DIR, src + ".o")
-        cmd = [hipcc, "-x", "hip"] + [f for f in FLAGS if f != "-shared"] + \
-              ["-c", os.path.join(CSRC, src), "-o", obj]
+
+    def start(cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
-        procs.append((src, subprocess.Popen(cmd)))
-        objs.append(obj)
-    cmd = torch_ops_command(TORCH_OPS_PATH)
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    procs.append((TORCH_OPS, subprocess.Popen(cmd)))
-    for src, p in procs:
-        if p.wait() != 0:
-            raise RuntimeError(f"the compiler failed on {src}")
-    cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+        return subprocess.Popen(cmd)
+
+    torch_ops = None
+    if module:
+        # (never one of other sources beside the library: it relies on the header's signatures)
+        if os.path.exists(TORCH_OPS_PATH):
+            os.remove(TORCH_OPS_PATH)
+        try:
+            torch_ops = start(torch_ops_command(TORCH_OPS_PATH))
+        except (ImportError, OSError) as e:
+            print(e, file=sys.stderr)
+    if library:
+        objs = [os.path.join(LIB_DIR, src + ".o") for src in SOURCES]
+        procs = [start([hipcc, "-x", "hip"] + [f for f in FLAGS if f != "-shared"] + ["-c", os.path.join(CSRC, src), "-o", obj])
+                 for src, obj in zip(SOURCES, objs)]
+        failed = [src for src, p in zip(SOURCES, procs) if p.wait() != 0]
+        if failed:
+            raise RuntimeError(f"the compiler failed on {', '.join(failed)}")
+        if start([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs).wait() != 0:
+            raise RuntimeError("linking the library failed")
+    if module and (torch_ops is None or torch_ops.wait() != 0):
+        raise RuntimeError(f"the compiler failed on {TORCH_OPS}: the library is complete, but embedding_lookup, list_logps, "
+                           "preference_loss and FusedAdamW will not run")
     return LIB_PATH
 
 
