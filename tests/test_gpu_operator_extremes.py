@@ -1,9 +1,12 @@
 """The embedding, list and AdamW operators at the far ends of what they accept, and in the calls that programs make
 around them: other streams and threads, repeated backward passes, transforms of torch.func."""
+import threading
+
 import pytest
 import torch
 
-from recommend_amd import ops
+from recommend_amd import _ffi, ops
+from recommend_amd.loss import list_logps, preference_loss
 from recommend_amd.optim import FusedAdamW
 from recommend_amd.train_step import GraphedTrainStep
 
@@ -105,3 +108,131 @@ def test_a_late_parameter_is_corrected_with_the_common_count():
     move = 1e-2 / (1 - 0.9 ** 21) * 0.1 / (0.001 / (1 - 0.999 ** 21)) ** 0.5
     assert int(opt.step_count) == 21
     assert float((late.detach().double() - (1 - move)).abs().max()) <= (16 * move + 1) * 2.0 ** -24
+
+
+def inputs(seed, n=700, rows=900):
+    """Of a lookup with gradient (counting sort) and of a preference step."""
+    g = torch.Generator().manual_seed(seed)
+    table, grad = torch.randn(rows, 64, generator=g).to(DEV), torch.randn(n, 64, generator=g).to(DEV)
+    scores = torch.randn(8, 3, 5000, generator=g).to(DEV)
+    items, ref = torch.randint(5000, (8, 3), generator=g).to(DEV), torch.randn(8, generator=g).to(DEV)
+    return table, torch.randint(rows, (n,), generator=g).to(DEV), grad, scores, items, ref
+
+
+def both(table, ids, grad, scores, items, ref):
+    table, scores = table.requires_grad_(True), scores.requires_grad_(True)
+    out = ops.embedding_lookup(table, ids, scale=1.5, padding_idx=0)
+    loss, logps = preference_loss(scores, items, ref)
+    return [out.detach(), torch.autograd.grad(out, table, grad)[0], loss.detach(), logps.detach(), torch.autograd.grad(loss, scores)[0]]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_second_backward_pass_with_the_graph_retained():
+    table, ids, grad, scores, items, ref = inputs(1)
+    want = both(table, ids, grad, scores, items, ref)
+    out, (loss, _) = ops.embedding_lookup(table, ids, scale=1.5, padding_idx=0), preference_loss(scores, items, ref)
+    for _ in range(2):
+        assert torch.equal(torch.autograd.grad(out, table, grad, retain_graph=True)[0], want[1])
+        assert torch.equal(torch.autograd.grad(loss, scores, retain_graph=True)[0], want[4])
+    for y, x, g in ((out, table, grad), (loss, scores, None)):
+        torch.autograd.grad(y, x, g)
+        with pytest.raises(RuntimeError, match="second time|freed"):
+            torch.autograd.grad(y, x, g)
+
+
+def test_inputs_changed_between_the_passes_are_refused():
+    table, ids, grad, scores, items, ref = inputs(2)
+    out, (loss, _) = (ops.embedding_lookup(table.requires_grad_(True), ids),
+                      preference_loss(scores.requires_grad_(True), items, ref))
+    ids.add_(0)
+    items.add_(0)
+    for y, x, g in ((out, table, grad), (loss, scores, None)):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, x, g)
+
+
+def test_on_another_stream_than_the_default_one():
+    """Forward and backward on a side stream behind slow work, without a wait by the host."""
+    args = inputs(3)
+    want = both(*args)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        slow = torch.randn(4096, 4096, device=DEV)
+        late = [torch.zeros_like(a) for a in args]
+        for _ in range(20):
+            slow = slow @ slow / 64
+        for a, b in zip(late, args):
+            with torch.no_grad():
+                a.copy_(b)
+        got = both(*[a.detach() for a in late])
+        p, q = (torch.nn.Parameter(args[0].detach().clone()) for _ in range(2))
+        p.grad = late[2][:1].expand(900, 64).contiguous()
+        FusedAdamW([p], lr=0.1, max_grad_norm=1.0).step()
+    torch.cuda.current_stream().wait_stream(side)
+    q.grad = args[2][:1].expand(900, 64).contiguous()
+    FusedAdamW([q], lr=0.1, max_grad_norm=1.0).step()
+    assert same(got, want) and torch.equal(p, q)
+
+
+def test_from_several_threads_at_once():
+    cases = [inputs(10 + k, n=300 + 400 * k) for k in range(4)]
+    want = [both(*c) for c in cases]
+    params = [torch.nn.Parameter(c[0].detach().clone()) for c in cases]
+    twins = [torch.nn.Parameter(c[0].detach().clone()) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                opt = FusedAdamW([params[k]], lr=1e-2, max_grad_norm=1.0, state_bits=8 if k % 2 else 32)
+                for _ in range(20):
+                    got = both(*cases[k])
+                    params[k].grad = got[1]
+                    opt.step()
+                    torch.cuda.current_stream().synchronize()
+                    if not same(got, want[k]):
+                        wrong.append(k)
+        except Exception as e:                            # (seen by the test, not only by the thread)
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for k, (p, q) in enumerate(zip(params, twins)):
+        opt = FusedAdamW([q], lr=1e-2, max_grad_norm=1.0, state_bits=8 if k % 2 else 32)
+        for _ in range(20):
+            q.grad = want[k][1]
+            opt.step()
+        assert torch.equal(p, q)
+
+
+def test_transforms_and_tensors_without_memory_raise():
+    """grad, vmap and jvp of torch.func, and fake tensors, hand over tensors whose memory cannot be read."""
+    table, ids, grad, scores, items, ref = inputs(4)
+    calls = (lambda t, i, s, y: ops.embedding_lookup(t, i).sum(), lambda t, i, s, y: list_logps(s, y).sum(),
+             lambda t, i, s, y: preference_loss(s, y, ref)[0])
+    args = (table, ids, scores, items)
+    for f, over in zip(calls, (0, 2, 2)):
+        with pytest.raises((RuntimeError, NotImplementedError, _ffi.RkError)):
+            torch.func.grad(f, argnums=over)(*args)
+        with pytest.raises((RuntimeError, NotImplementedError, _ffi.RkError)):
+            torch.func.jvp(lambda x: f(*args[:over], x, *args[over + 1:]), (args[over],), (args[over],))
+        for which in (over, over + 1):
+            dims = tuple(0 if k == which else None for k in range(4))
+            batched = [torch.stack([a, a]) if k == which else a for k, a in enumerate(args)]
+            with pytest.raises((RuntimeError, NotImplementedError, _ffi.RkError)):
+                torch.func.vmap(f, in_dims=dims)(*batched)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        fake = [mode.from_tensor(a) for a in args]
+        for f in calls[:2]:
+            with pytest.raises((RuntimeError, NotImplementedError, _ffi.RkError)):
+                f(*fake)
