@@ -34,9 +34,6 @@ class AdamTensor(Structure):
                 ("n", c_int64)]
 
 
-# element types of the entry points that take more than fp32 (RK_F32, RK_BF16, RK_F16)
-F32, BF16, F16 = 0, 1, 2
-
 ADAMW_BLOCK = 64
 ADAMW_MAX_GROUPS = 8
 
