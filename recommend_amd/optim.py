@@ -37,6 +37,7 @@ class FusedClipAdam(torch.optim.Optimizer):
         self._group = group
         self._all_reduce = all_reduce    # all_reduce(tensor, group): sums in place (default: torch.distributed)
         self._tables = {}        # pointer set -> (descriptor array, workspace, replicated count)
+        self._held = []          # memory that a step recorded in a HIP graph may go on using
         self._dev = None
         self._lr_host = None
         self._restored_step = None
@@ -45,6 +46,7 @@ class FusedClipAdam(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._tables = {}
+        self.__dict__.setdefault("_held", [])
 
     def _state_for(self, p):
         st = self.state[p]
@@ -97,6 +99,8 @@ class FusedClipAdam(torch.optim.Optimizer):
         if self._dev is None:
             self._init_device(params[0].device)
         arr, ws, n_rep = self._prepare(params)     # (moments are created outside any graph capture: first eager step)
+        if torch.cuda.is_current_stream_capturing():
+            self._held.append(ws)                  # (the table that holds it may go before the graph does)
         if self._lr_host != group["lr"]:
             if torch.cuda.is_current_stream_capturing():
                 if self._lr_host is None:
@@ -138,20 +142,24 @@ class FusedClipAdam(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Moments and step count of a checkpoint (this optimizer's or torch.optim.Adam's).  Moment
-        buffers that exist already keep their memory and take the checkpoint's VALUES, so a training
-        step recorded in a HIP graph before the load (its kernels hold the buffers' addresses) goes on
-        updating the moments the optimizer reports; the learning rate of the checkpoint reaches the
-        device scalar at once for the same reason.  Call it outside graph capture."""
+        buffers that exist already keep their memory and take the checkpoint's VALUES (zeros, where it has
+        none for their parameter), so a training step recorded in a HIP graph before the load (its kernels
+        hold the buffers' addresses) goes on updating the moments the optimizer reports; the learning rate of
+        the checkpoint reaches the device scalar at once for the same reason.  Call it outside graph capture."""
         old = {p: (st["exp_avg"], st["exp_avg_sq"]) for p, st in self.state.items() if "exp_avg" in st}
         super().load_state_dict(state_dict)
         for q, (m, v) in old.items():
             st = self.state.get(q)
             if st is None or "exp_avg" not in st:
-                continue
-            if st["exp_avg"].shape == m.shape and st["exp_avg"].device == m.device:
+                m.zero_()
+                v.zero_()
+                self.state[q] = {"exp_avg": m, "exp_avg_sq": v}
+            elif st["exp_avg"].shape == m.shape and st["exp_avg"].device == m.device:
                 m.copy_(st["exp_avg"])
                 v.copy_(st["exp_avg_sq"])
                 st["exp_avg"], st["exp_avg_sq"] = m, v
+            else:
+                self._held += [m, v]
         self._tables = {}        # descriptor tables are rebuilt from the state at the next step
         steps = [float(st["step"]) for st in self.state.values() if "step" in st]
         self._restored_step = int(max(steps)) if steps else 0

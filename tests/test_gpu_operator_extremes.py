@@ -7,7 +7,7 @@ import torch
 
 from recommend_amd import _ffi, ops
 from recommend_amd.loss import list_logps, preference_loss
-from recommend_amd.optim import FusedAdamW
+from recommend_amd.optim import FusedAdamW, FusedClipAdam
 from recommend_amd.train_step import GraphedTrainStep
 
 pytestmark = pytest.mark.gpu
@@ -35,14 +35,16 @@ def test_rows_whose_vectors_pass_32_bits(dtype, D, n):
     assert torch.equal(dw[1], 2 * grad[0] if n else torch.zeros_like(dw[1]))
 
 
-@pytest.mark.parametrize("bits", [8, 32])
-def test_recorded_step_goes_on_after_a_checkpoint_without_its_moments(bits):
+@pytest.mark.parametrize("make", [lambda p: FusedAdamW(p, lr=1e-2, max_grad_norm=1.0, state_bits=8),
+                                  lambda p: FusedAdamW(p, lr=1e-2, max_grad_norm=1.0),
+                                  lambda p: FusedClipAdam(p, lr=1e-2, max_grad_norm=1.0)], ids=["8", "32", "clip"])
+def test_recorded_step_goes_on_after_a_checkpoint_without_its_moments(make):
     """A step is recorded, then the checkpoint from before the first step is loaded: replays do what a new optimizer
     does, and touch nothing that was allocated since."""
     g = torch.Generator().manual_seed(5)
     start = [torch.randn(s, generator=g).to(DEV) for s in ((100, 64), (64,))]
     ours = [torch.nn.Parameter(w.clone()) for w in start]
-    opt = FusedAdamW(ours, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+    opt = make(ours)
     saved = opt.state_dict()
     for p in ours:
         p.grad = torch.randn(p.shape, generator=g).to(DEV)
@@ -56,10 +58,10 @@ def test_recorded_step_goes_on_after_a_checkpoint_without_its_moments(bits):
     with torch.no_grad():
         for p, w in zip(ours, start):
             p.copy_(w)
-    # every size that a moment has had: freed ones would be given out here
-    others = [torch.full((n,), 7, dtype=torch.uint8, device=DEV) for n in (6400, 25600, 400, 256) for _ in range(20)]
+    # every size that a moment or a workspace has had: freed ones would be given out here
+    others = [torch.full((n,), 7, dtype=torch.uint8, device=DEV) for n in (6400, 25600, 400, 256, 32) for _ in range(20)]
     fresh = [torch.nn.Parameter(w.clone()) for w in start]
-    same = FusedAdamW(fresh, lr=1e-2, max_grad_norm=1.0, state_bits=bits)
+    same = make(fresh)
     for k in range(4):
         for p, q in zip(ours, fresh):
             p.grad.copy_(torch.randn(p.shape, generator=g))

@@ -1,9 +1,9 @@
-"""What FusedAdamW's load_state_dict does to the moments that exist, on the host: a step recorded in a HIP graph holds
-their addresses, so no load may free them."""
+"""What load_state_dict of FusedAdamW and FusedClipAdam does to the moments that exist, on the host: a step recorded in a
+HIP graph holds their addresses, so no load may free them."""
 import pytest
 import torch
 
-from recommend_amd.optim import FusedAdamW, encode_moment
+from recommend_amd.optim import FusedAdamW, FusedClipAdam, encode_moment
 
 
 def optimizer(bits, shapes=((100, 64), (64,), ())):
@@ -90,3 +90,19 @@ def test_counts_that_differ_continue_with_the_largest():
     opt = FusedAdamW([torch.nn.Parameter(torch.ones(3)) for _ in range(2)])
     opt.load_state_dict(theirs.state_dict())
     assert opt._restored_step == 4
+
+
+def test_clip_adam_keeps_moments_that_the_checkpoint_lacks():
+    params = [torch.nn.Parameter(torch.ones(n)) for n in (5, 6, 7)]
+    opt = FusedClipAdam(params)
+    for p in params:
+        opt.state[p].update(exp_avg=torch.full_like(p, 2.0), exp_avg_sq=torch.full_like(p, 3.0), step=torch.tensor(3.0))
+    held = [addresses(opt, p) for p in params]
+    partial = opt.state_dict()
+    partial["state"] = {1: {k: v.clone() for k, v in partial["state"][1].items()}}
+    opt.load_state_dict(partial)
+    assert [addresses(opt, p) for p in params] == held
+    assert cleared(opt, params[0]) and cleared(opt, params[2]) and bool((opt.state[params[1]]["exp_avg"] == 2).all())
+    opt.load_state_dict(FusedClipAdam([torch.nn.Parameter(torch.ones(n)) for n in (5, 6, 7)]).state_dict())
+    assert [addresses(opt, p) for p in params] == held and all(cleared(opt, p) for p in params)
+    assert opt._restored_step == 0
