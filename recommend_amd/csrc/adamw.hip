@@ -9,7 +9,7 @@
 // sum per workgroup.  The next one, a single workgroup, advances the step count, joins the partial sums
 // in order and leaves the step's factors in the workspace.  The last one updates.  (Joining in the
 // workgroup that finishes the norm last saves the small launch, but its release fences write back the
-// L2 once per workgroup: 158 us instead of 60 for 185 MB.)  The descriptors travel by value in the kernels' arguments
+// L2 once per workgroup: 158 us instead of 60 for 167 MB.)  The descriptors travel by value in the kernels' arguments
 // (kMaxTensors per launch): nothing is copied or allocated, so a step can be recorded in a HIP graph.
 //
 // 8-bit moments: blocks of 64 consecutive elements share an fp32 scale; m and the root of v are held as

@@ -6,8 +6,7 @@
 // lane groups add them in registers in that order and write each row of dW once.  The sums are fp32
 // whatever the tensors' type, the same bits on every run, and rounded once.
 //
-// Up to kFewIds ids one launch does all of it (512 ids of width 64, 7050 rows: 12 us; the three launches
-// below 3 + 5 + 4 and the gaps between them, and two launches more for the host).  Otherwise:
+// Up to kFewIds ids one launch does all of it.  Otherwise:
 // Sort: up to kRankSortMax ids one launch counts, for every id, the ids that come before it.  More
 // ids take an LSD radix sort with digits of up to 9 bits: per digit one launch that counts every
 // tile's digits, one that adds up each digit's counts over the tiles and one that places the ids.
@@ -24,14 +23,19 @@
 
 namespace {
 
-constexpr int kRankSortMax = 8192;    // ids sorted by counting
+// Ids sorted by counting, in one launch whose work grows with their square (whole gradient of 7050 x 64 floats, counting /
+// radix sort: 15 / 35 us for 2048 ids, 30 / 41 for 8192, 59 / 43 for 12288).
+constexpr int kRankSortMax = 8192;
 constexpr int kRankThreads = 16;      // threads that count for one id
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / rk::kWave;
 constexpr int kMaxDigitBits = 9;      // one thread for each digit
 constexpr int kTileSteps = 8;         // ids of a thread: they stay in registers
 constexpr int kTile = kSortThreads * kTileSteps;
-constexpr int kFewBits = 9, kFewIds = 1 << kFewBits;   // ids that every summing workgroup sorts itself: one launch
+// Ids that every summing workgroup sorts itself: one launch instead of three (gradient of 7050 x 64 floats: 3.8 / 6.6 us
+// for 16 ids, 7.7 / 10.0 for 256, 11.9 / 11.7 for 512, 17.8 / 12.2 for 640; of 255404 x 128 bf16 14.2 / 19.0 for 512 and
+// 20.2 / 19.5 for 640).
+constexpr int kFewBits = 9, kFewIds = 1 << kFewBits;
 constexpr int32_t kFewRows = 1 << (32 - kFewBits);      // (key and position have to fit a word)
 constexpr int kMaxEntries = 1024;     // sorted entries of one workgroup of the summing launch
 constexpr int kZeroRows = 256;        // rows that a zeroing workgroup looks up together
@@ -39,11 +43,17 @@ constexpr int kZeroRows = 256;        // rows that a zeroing workgroup looks up 
 // million rows of 8 floats: 403 us with four blocks, 579 with one; in 2.2 million rows 53 and 67).
 constexpr int kZeroSteps = 4;
 constexpr int32_t kManyRows = 2048 * kZeroSteps * kZeroRows;
-constexpr int kPerGroup = 32;         // sorted entries of a lane group
+// Sorted entries of a lane group (whole gradient of 2^20 ids, one of them everywhere, 128 bf16: 207 us with 16, 159 with
+// 32, 161 with 64; skewed ids 122 with each; 131072 ids of 1024 floats 210, 191 and 186).
+constexpr int kPerGroup = 32;
 constexpr int kJoinLanes = 64;       // lanes of a row in the closing launch, at most
-constexpr int kJoins = 4;             // workgroup borders that one workgroup of the closing launch looks at
+// Workgroup borders that one workgroup of the closing launch looks at (8192 ids: 29.6 us with one, 30.0 with four, 31.8
+// with 16; 131072 ids of 1024 floats 202, 191 and 191).
+constexpr int kJoins = 4;
 constexpr int64_t kStreamBytes = 64 << 20;   // looked-up rows from this size on are stored past the caches
-constexpr int kLongRun = 8;          // workgroup pieces of a row above which a whole workgroup joins them
+// Workgroup pieces of a row above which a whole workgroup joins them (2^20 skewed ids: 130 us with one, 122 with eight,
+// 129 with 32; 8192 ids 40, 30 and 30).
+constexpr int kLongRun = 8;
 
 // the sort key of an id: ids outside [0, rows) and the padding id go behind all rows
 template <typename ID>

@@ -21,7 +21,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / rk::kWave;
 constexpr int kPairThreads = 1024;
-constexpr int kFewRows = 4096;       // rows that one workgroup joins
+// Rows that one workgroup joins, in the launch of the pairs: one launch fewer, which a call from the host notices (a step
+// over 4000 rows of 300 scores: 53 us, with two launches 57) and a recorded one does not (forward 13.5 us, 9.8).
+constexpr int kFewRows = 4096;
 // Pairs that one workgroup adds up behind more rows than that; more take two launches (4096 pairs 7.2 us, in two
 // launches 2.9 + 1.8 and a gap; 100000 pairs 129 us, 4.9 + 4.7).
 constexpr int kOnePairs = 4096;
@@ -459,7 +461,8 @@ void cut(Rows &a, int want_blocks) {
 // forward 94 / 294 (200000 rows of 100 scores), 47 / 126 (100000 of 1000), 38 / 52 (30000 of 4000), 6.0 / 7.2
 // (2000 of 4000); backward 73 / 186, 61 / 96, 4.5 / 5.2 (2000 of 1000), 7.1 / 5.8 (2000 of 2000).
 constexpr int kWaveFwd = 4096, kWaveBwd = 1024;
-// (few parts: the longer ones by a workgroup, 4.0 us instead of 4.4 for 16 parts of 3525)
+// (few parts: the longer ones by a workgroup.  Whole forward calls over rows of 4096 scores, by a workgroup / by a wavefront:
+// 7.4 / 7.6 us for 2 rows, 7.7 / 8.3 for 16, 8.4 / 8.7 for 400, 9.9 / 9.6 for 1000, 12.8 / 11.5 for 2000)
 bool fwd_by_wave(const Rows &a) { return a.part_len <= (a.units >= 1024 ? kWaveFwd : kWaveFwd / 2); }
 
 dim3 grid_of(const Rows &a, bool by_wave) {
