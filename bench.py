@@ -45,9 +45,13 @@ METRICS = ["precision", "recall", "hit_rate", "ndcg", "map", "mrr"]
 K_LIST = [5, 10, 20]
 HBM_PEAK_GBS = 8000.0        # MI355X HBM3E spec
 # Memory-side bytes per launch come from rocprofv3 PMC passes over THIS program (`--pmc-pass`, one
-# counter per run: tools/pmc_bench.sh), summarised by tools/pmc_traffic.py into the newest
-# profiles/r*_pmc_traffic.json.  The summary names the workload and a digest of the kernel sources it
-# was collected from; a line measured on another workload or on changed sources reports null.
+# counter per run: tools/pmc_bench.sh), summarised by tools/pmc_traffic.py into
+# profiles/bench_pmc_traffic.json.  The summary names the workload and a digest of the kernels it
+# was collected from; a line measured on another workload or on changed kernels reports null.
+TRAFFIC = os.path.join("profiles", "bench_pmc_traffic.json")
+# what the kernels of a top-K call and of an SpMM hop are compiled from
+TRAFFIC_SOURCES = ("common.h", "eval.hip", "eval_filter.hip", "spmm.hip", "topk_filter.h", "topk_kernel.h",
+                   "topk_threshold.h", "topk_wide.h")
 MFMA_F32_PEAK_TFS = 157.3    # MI355X fp32 matrix peak
 MFMA_F16_PEAK_TFS = 2500.0   # MI355X dense fp16 / bf16 matrix peak
 BATCH = {"baby": 2048, "clothing": 1024, "sports": 256, "elec": 256}   # reference config.py presets
@@ -56,32 +60,31 @@ LR = {"baby": 1e-3, "clothing": 5e-4, "sports": 1e-3, "elec": 1e-3}    # config.
 
 
 def kernel_source_digest():
-    """sha256 over the kernel sources, so counter summaries can be tied to the code they measured."""
-    import glob
+    """sha256 over the sources and compiler flags of the kernels whose traffic is reported, so counter
+    summaries can be tied to the code they measured."""
     import hashlib
-    h = hashlib.sha256()
-    for f in sorted(glob.glob(os.path.join(ROOT, "recommend_amd", "csrc", "*"))):
-        if f.endswith((".hip", ".h", ".cpp")):
-            h.update(os.path.basename(f).encode())
-            h.update(open(f, "rb").read())
+    from recommend_amd.build import FLAGS
+    h = hashlib.sha256(" ".join(FLAGS).encode())
+    for name in TRAFFIC_SOURCES:
+        h.update(name.encode())
+        with open(os.path.join(ROOT, "recommend_amd", "csrc", name), "rb") as f:
+            h.update(f.read())
     return h.hexdigest()[:16]
 
 
 def pmc_traffic(group, shape, D, world):
-    """(bytes per launch, file it came from) of a kernel group from the newest counter summary, or
-    (None, reason) when there is none for this workload and these sources."""
-    import glob
-    files = sorted(glob.glob(os.path.join(ROOT, "profiles", "r*_pmc_traffic.json")))
-    if not files:
-        return None, "no profiles/r*_pmc_traffic.json"
-    name = os.path.relpath(files[-1], ROOT)
-    with open(files[-1]) as f:
+    """(bytes per launch, file it came from) of a kernel group from the counter summary, or
+    (None, reason) when there is none for this workload and these kernels."""
+    path = os.path.join(ROOT, TRAFFIC)
+    if not os.path.exists(path):
+        return None, f"no {TRAFFIC}"
+    with open(path) as f:
         doc = json.load(f)
     if doc.get("shape") != shape or doc.get("emb_dim") != D or world != 1:
-        return None, f"{name} was collected on {doc.get('shape')} / emb_dim {doc.get('emb_dim')} / 1 GPU"
+        return None, f"{TRAFFIC} was collected on {doc.get('shape')} / emb_dim {doc.get('emb_dim')} / 1 GPU"
     if doc.get("kernel_source_digest") != kernel_source_digest():
-        return None, f"{name} was collected from other kernel sources ({doc.get('kernel_source_digest')})"
-    return doc["groups"][group]["traffic_bytes"], name
+        return None, f"{TRAFFIC} was collected from other kernel sources ({doc.get('kernel_source_digest')})"
+    return doc["groups"][group]["traffic_bytes"], TRAFFIC
 
 
 def log(*a):

@@ -26,5 +26,5 @@ run sq_proj $SQ -- python3 $root/tools/proj_probe.py
 run grbm GRBM_GUI_ACTIVE -- $B
 grep -h '^{' $out/fetch.log | tail -1 > $out/bench_line.json
 # only the summaries travel back (the per-dispatch tables are tens of MB)
-python3 $root/tools/pmc_traffic.py $out $keep/r
+python3 $root/tools/pmc_traffic.py $out $keep/bench
 cp $out/bench_line.json $out/*.log $keep/
