@@ -169,7 +169,8 @@ class FusedClipAdam(torch.optim.Optimizer):
         self.sync_lr()
 
     def sync_lr(self):
-        """Push a learning rate changed by a scheduler to the device scalar (call outside graph capture)."""
+        """Push a learning rate changed by a scheduler to the device scalar.  step() does it, and so do the recorded steps
+        of train_step and dist_train; call it before replaying a graph of your own, outside the capture."""
         lr = self.param_groups[0]["lr"]
         if self._dev is not None and self._lr_host != lr:
             self.lr_dev.fill_(float(lr))
@@ -335,8 +336,8 @@ class FusedAdamW(torch.optim.Optimizer):
                                            self.grad_norm, self._ws)
 
     def sync_lr(self):
-        """Push learning rates changed by a scheduler to device memory (step() does it; call it for a step that
-        is replayed from a graph, outside the capture)."""
+        """Push learning rates changed by a scheduler to device memory.  step() does it, and so do the recorded steps
+        of train_step and dist_train; call it before replaying a graph of your own, outside the capture."""
         rates = [float(g["lr"]) for g in self.param_groups]
         if self._dev is None or rates == self._rates:
             return

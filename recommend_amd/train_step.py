@@ -40,12 +40,15 @@ class GraphedStep:
 
     def __init__(self, body: Callable[[Dict], torch.Tensor], zero_grad: Callable[[], None],
                  example_batch: Dict[str, torch.Tensor], constants: Optional[Dict[str, torch.Tensor]] = None,
-                 warmup_steps: int = 3, capture: bool = True, capture_error_mode: str = "global"):
+                 warmup_steps: int = 3, capture: bool = True, capture_error_mode: str = "global",
+                 before_step: Optional[Callable[[], None]] = None):
+        """before_step: called before every step behind the capture, outside of it (what the recorded kernels read
+        from device memory and the program keeps on the host: learning rates)."""
         if warmup_steps < 1:
             # optimizers create their state on the first step; created inside the capture it would
             # be re-zeroed by every replay
             raise ValueError("at least one eager warm-up step is needed before the capture")
-        self._body_fn, self._zero_grad = body, zero_grad
+        self._body_fn, self._zero_grad, self._before_step = body, zero_grad, before_step
         dev = next(iter(example_batch.values())).device
         self.constants = dict(constants or {})
         self.static = {k: v.clone() for k, v in example_batch.items() if k not in self.constants}
@@ -81,6 +84,8 @@ class GraphedStep:
     def __call__(self, batch: Dict[str, torch.Tensor]) -> torch.Tensor:
         """Runs one step on `batch`; returns the loss (a device scalar that the next call
         overwrites)."""
+        if self._before_step is not None:
+            self._before_step()
         if self.graph is None or any(tuple(batch[k].shape) != self.shapes[k] for k in self.shapes):
             # on the stream the recorded step's autograd nodes were created on (gradient accumulators
             # outlive an iteration and remember their stream)
@@ -112,8 +117,9 @@ class GraphedTrainStep(GraphedStep):
         # (FusedClipAdam and FusedAdamW of recommend_amd.optim clip inside their own updates)
         self.max_grad_norm, self._opt_clips = clip_norm(optimizer, max_grad_norm)
         self.params = [p for p in model.parameters() if p.requires_grad]
+        # (sync_lr: a rate that a scheduler changed reaches the recorded step)
         super().__init__(self._train_body, lambda: self.opt.zero_grad(set_to_none=True), example_batch, constants,
-                         warmup_steps)
+                         warmup_steps, before_step=getattr(optimizer, "sync_lr", None))
 
     def _train_body(self, batch):
         loss = self.loss_fn(self.model(batch), batch)

@@ -238,3 +238,26 @@ def test_transforms_and_tensors_without_memory_raise():
         for f in calls[:2]:
             with pytest.raises((RuntimeError, NotImplementedError, _ffi.RkError)):
                 f(*fake)
+
+
+@pytest.mark.parametrize("make", [FusedAdamW, FusedClipAdam])
+def test_recorded_training_step_follows_a_scheduler(make):
+    g = torch.Generator().manual_seed(8)
+    net = torch.nn.Module()
+    net.weight = torch.nn.Parameter(torch.randn(64, generator=g).to(DEV))
+    net.forward = lambda b: b["x"] * net.weight
+    batches = [{"x": torch.randn(32, 64, generator=g).to(DEV)} for _ in range(6)]
+    twin = torch.nn.Parameter(net.weight.detach().clone())
+    opt, same = make([net.weight], lr=0.1, max_grad_norm=1.0), make([twin], lr=0.1, max_grad_norm=1.0)
+    step = GraphedTrainStep(net, opt, lambda out, b: out.square().mean(), batches[0], warmup_steps=1)
+    rates = [torch.optim.lr_scheduler.StepLR(o, 2, gamma=0.3) for o in (opt, same)]
+    for k, b in enumerate([batches[0]] + batches):
+        if k > 0:
+            step(b)
+        twin.grad, = torch.autograd.grad((b["x"] * twin).square().mean(), twin)
+        same.step()
+        for r in rates:
+            r.step()
+        torch.cuda.synchronize()
+        assert torch.equal(net.weight, twin), k
+    assert opt.param_groups[0]["lr"] < 0.01
