@@ -268,11 +268,17 @@ class FusedAdamW(torch.optim.Optimizer):
             if len({id(p[1] if isinstance(p, tuple) else p) for p in params}) != len(params):
                 raise ValueError("FusedAdamW: a parameter appears twice in a group")
             group = {**group, "params": params}
+        self._check_group({**self.defaults, **group})
         super().add_param_group(group)
-        g = self.param_groups[-1]
+
+    @staticmethod
+    def _check_group(g):
         b1, b2 = g["betas"]
         if not (0 <= b1 < 1 and 0 <= b2 < 1 and g["eps"] >= 0 and g["weight_decay"] >= 0 and g["lr"] >= 0):
             raise ValueError("FusedAdamW: betas in [0, 1), eps, weight_decay and lr not negative")
+        for other in ("amsgrad", "maximize"):
+            if g.get(other):
+                raise ValueError(f"FusedAdamW: {other} is not built")
 
     def __getstate__(self):
         steps = int(self.step_count.item()) if self._dev is not None else self._restored_step
@@ -395,6 +401,8 @@ class FusedAdamW(torch.optim.Optimizer):
         old = {p: {k: v for k, v in st.items() if k != "step" and torch.is_tensor(v)} for p, st in self.state.items()}
         # (torch casts floating state to the parameter's type on the way: the values are taken from the checkpoint
         # itself, and before anything is replaced, so that a checkpoint of other sizes leaves all as it was)
+        for g in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **g})
         fresh = self._moments_of(state_dict)
         super().load_state_dict(state_dict)
         for p, st in fresh.items():

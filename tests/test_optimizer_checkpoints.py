@@ -106,3 +106,30 @@ def test_clip_adam_keeps_moments_that_the_checkpoint_lacks():
     opt.load_state_dict(FusedClipAdam([torch.nn.Parameter(torch.ones(n)) for n in (5, 6, 7)]).state_dict())
     assert [addresses(opt, p) for p in params] == held and all(cleared(opt, p) for p in params)
     assert opt._restored_step == 0
+
+
+@pytest.mark.parametrize("other", ["amsgrad", "maximize"])
+def test_other_updates_than_the_built_one_are_refused(other):
+    """torch's AdamW with them takes other steps: neither its checkpoints nor groups that ask for them pass in silence."""
+    w = torch.nn.Parameter(torch.ones(3))
+    theirs = torch.optim.AdamW([w], **{other: True})
+    w.grad = torch.ones(3)
+    theirs.step()
+    opt, params = optimizer(32, ((3,),))
+    held = addresses(opt, params[0])
+    with pytest.raises(ValueError, match=other):
+        opt.load_state_dict(theirs.state_dict())
+    assert addresses(opt, params[0]) == held and opt.param_groups[0]["lr"] == 1e-3
+    with pytest.raises(ValueError, match=other):
+        FusedAdamW([{"params": [w], other: True}])
+    bad = torch.optim.AdamW([w]).state_dict()
+    bad["param_groups"][0]["betas"] = (0.9, 1.0)
+    with pytest.raises(ValueError, match="betas"):
+        opt.load_state_dict(bad)
+
+
+def test_a_refused_group_is_not_added():
+    opt, _ = optimizer(32, ((3,),))
+    with pytest.raises(ValueError, match="betas"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2))], "betas": (0.9, 1.0)})
+    assert len(opt.param_groups) == 1
