@@ -18,7 +18,7 @@ python3 - $out > $keep/r03_pmc_scaleup_slices.txt <<'PY'
 import csv, sys, collections
 src = sys.argv[1]
 print("SpMM hop on one rank's row block of the 10M x 2M x 500M configuration (D = 128), memory-side traffic per launch:")
-print("FETCH_SIZE / WRITE_SIZE in KB, mean over the launches of spmm_rows_kernel; bytes = 1000 * (2 * FETCH_SIZE + WRITE_SIZE)")
+print("FETCH_SIZE / WRITE_SIZE in units of 1024 bytes, mean over the launches of spmm_rows_kernel; bytes = 1024 * (2 * FETCH_SIZE + WRITE_SIZE)")
 print("(gfx950 tallies its 128-B read requests at 64 B)\n")
 for rank in (0, 7):
     tot = {}
@@ -31,7 +31,7 @@ for rank in (0, 7):
         tot["n"] = n
     log = [l.strip() for l in open(f"{src}/r{rank}_FETCH_SIZE.log") if "block of rank" in l or "local SpMM" in l]
     print(f"rank {rank}: {tot['n']} launches, FETCH_SIZE {tot['FETCH_SIZE']:.0f} KB, WRITE_SIZE {tot['WRITE_SIZE']:.0f} KB "
-          f"-> {1e3 * (2 * tot['FETCH_SIZE'] + tot['WRITE_SIZE']) / 1e9:.2f} GB per launch")
+          f"-> {1024 * (2 * tot['FETCH_SIZE'] + tot['WRITE_SIZE']) / 1e9:.2f} GB per launch")
     for l in log:
         print("   " + l)
 PY

@@ -4,7 +4,8 @@
 
 writes <prefix>_pmc_traffic.json (memory-side bytes per launch of the SpMM hop and of one fused
 top-K call, read by bench.py) and <prefix>_pmc_sq_summary.txt (SQ busy / MFMA-busy / VALU-busy
-per kernel).  FETCH_SIZE and WRITE_SIZE are in KB; on gfx950 FETCH_SIZE counts 128-B read
+per kernel).  FETCH_SIZE and WRITE_SIZE are in units of 1024 bytes (a kernel that reads 432.9 MB once shows
+2 * 211.4 thousand); on gfx950 FETCH_SIZE counts 128-B read
 requests at 64 B, so reads of 16 B per lane are doubled (all reads of these kernels are)."""
 import collections
 import csv
@@ -60,8 +61,8 @@ for table, key in ((fetch, "fetch_size_kb"), (write, "write_size_kb")):
 groups["score_topk_call"] = g
 for g in groups.values():
     g["fetch_size_kb"], g["write_size_kb"] = round(g["fetch_size_kb"], 1), round(g["write_size_kb"], 1)
-    g["traffic_bytes"] = round(1e3 * (2 * g["fetch_size_kb"] + g["write_size_kb"]))
-    g["formula"] = "1000 * (2 * FETCH_SIZE + WRITE_SIZE)"
+    g["traffic_bytes"] = round(1024 * (2 * g["fetch_size_kb"] + g["write_size_kb"]))
+    g["formula"] = "1024 * (2 * FETCH_SIZE + WRITE_SIZE)"
 doc = {"shape": line["config"]["workload"].split(" ")[0], "emb_dim": 64 if "emb_dim 64" in line["config"]["workload"] else 128,
        "kernel_source_digest": line["kernel_source_digest"], "command": "rocprofv3 --pmc <FETCH_SIZE | WRITE_SIZE> -- python3 bench.py --pmc-pass",
        "groups": groups}
