@@ -366,30 +366,42 @@ class FusedAdamW(torch.optim.Optimizer):
                     st["step"] = torch.tensor(t)
         return super().state_dict()
 
-    def _moments_of(self, state_dict):
-        """{parameter: its state} of a checkpoint, in the form this optimizer holds it."""
+    def _entries(self, state_dict):
+        """{parameter: its moments in the checkpoint}, checked: nothing is replaced by a checkpoint of other sizes."""
+        for g in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **g})
         saved, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             return {}                                # (another model's: torch says so)
-        fresh = {}
+        entries = {}
         for i, p in zip([i for g in groups for i in g["params"]], [p for g in self.param_groups for p in g["params"]]):
             src = saved.get(i)
             if not src or not ("exp_avg" in src or "exp_avg8" in src):
                 continue
-            src = {k: v.to(p.device) if torch.is_tensor(v) else v for k, v in src.items()}
-            st = {"step": torch.tensor(float(src.get("step", 0)))}
-            if self._is8(p) and "exp_avg8" in src:
-                st.update({k: src[k].clone() for k in _STATE8})
-            elif self._is8(p):
-                st["exp_avg8"], st["exp_avg8_scale"] = encode_moment(src["exp_avg"])
-                st["exp_avg_sq8"], st["exp_avg_sq8_scale"] = encode_moment(src["exp_avg_sq"].float().sqrt(), True)
-            elif "exp_avg" in src:
-                st.update({k: src[k].detach().float().reshape(p.shape).clone() for k in _STATE32})
-            else:
-                st["exp_avg"] = decode_moment(src["exp_avg8"], src["exp_avg8_scale"], p)
-                st["exp_avg_sq"] = decode_moment(src["exp_avg_sq8"], src["exp_avg_sq8_scale"], p).square()
-            fresh[p] = st
-        return fresh
+            n, blocks = p.numel(), -(-p.numel() // _ffi.ADAMW_BLOCK)
+            sizes = ((n, n) if "exp_avg" in src else
+                     (blocks * _ffi.ADAMW_BLOCK, blocks, blocks * _ffi.ADAMW_BLOCK, blocks))
+            for k, size in zip(_STATE32 if "exp_avg" in src else _STATE8, sizes):
+                if not torch.is_tensor(src.get(k)) or src[k].numel() != size:
+                    raise ValueError(f"FusedAdamW: {k} of a checkpoint does not fit a parameter of {tuple(p.shape)}")
+            entries[p] = src
+        return entries
+
+    def _moments_of(self, p, src):
+        """A parameter's state from a checkpoint's, in the form this optimizer holds it."""
+        src = {k: v.to(p.device) if torch.is_tensor(v) else v for k, v in src.items()}
+        st = {"step": torch.tensor(float(src.get("step", 0)))}
+        if self._is8(p) and "exp_avg8" in src:
+            st.update({k: src[k].clone() for k in _STATE8})
+        elif self._is8(p):
+            st["exp_avg8"], st["exp_avg8_scale"] = encode_moment(src["exp_avg"])
+            st["exp_avg_sq8"], st["exp_avg_sq8_scale"] = encode_moment(src["exp_avg_sq"].float().sqrt(), True)
+        elif "exp_avg" in src:
+            st.update({k: src[k].detach().float().reshape(p.shape).clone() for k in _STATE32})
+        else:
+            st["exp_avg"] = decode_moment(src["exp_avg8"], src["exp_avg8_scale"], p)
+            st["exp_avg_sq"] = decode_moment(src["exp_avg_sq8"], src["exp_avg_sq8_scale"], p).square()
+        return st
 
     def load_state_dict(self, state_dict):
         """Moments and step count of a checkpoint: this optimizer's with either number of bits, or
@@ -399,14 +411,15 @@ class FusedAdamW(torch.optim.Optimizer):
         with them.  Buffers of another form than the checkpoint's become are not used again, and not freed
         either.  Call it outside graph capture."""
         old = {p: {k: v for k, v in st.items() if k != "step" and torch.is_tensor(v)} for p, st in self.state.items()}
-        # (torch casts floating state to the parameter's type on the way: the values are taken from the checkpoint
-        # itself, and before anything is replaced, so that a checkpoint of other sizes leaves all as it was)
-        for g in state_dict["param_groups"]:
-            self._check_group({**self.defaults, **g})
-        fresh = self._moments_of(state_dict)
-        super().load_state_dict(state_dict)
-        for p, st in fresh.items():
-            held = old.pop(p, {})
+        entries = self._entries(state_dict)
+        # (torch would cast floating state to the parameter's type, all of it at once: the groups are its part, the
+        # moments are taken from the checkpoint itself, a parameter at a time)
+        super().load_state_dict({**state_dict, "state": {}})
+        for p, held in old.items():
+            if held:
+                self.state[p] = dict(held)
+        for p, src in entries.items():
+            st, held = self._moments_of(p, src), old.pop(p, {})
             for k, v in st.items():
                 have = held.get(k)
                 if have is not None and have.shape == v.shape and have.dtype == v.dtype:
@@ -414,12 +427,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     st[k] = held.pop(k)
             self._held += held.values()
             self.state[p] = st
-        for p, held in old.items():
-            if not held:
-                continue
+        for held in old.values():
             for v in held.values():
                 (v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v).zero_()
-            self.state[p] = held
         self._restored_step = max((int(st["step"]) for st in self.state.values() if "step" in st), default=0)
         if self._dev is not None:
             self.step_count.fill_(self._restored_step)

@@ -71,9 +71,9 @@ def test_a_checkpoint_of_other_sizes_leaves_everything_as_it_was():
     opt, params = optimizer(32)
     held = [addresses(opt, p) for p in params]
     values = [v.clone() for p in params for v in opt.state[p].values()]
-    other = optimizer(32, ((100, 64), (63,), ()))[0].state_dict()
-    with pytest.raises(RuntimeError):
-        opt.load_state_dict(other)
+    for bits in (8, 32):
+        with pytest.raises(ValueError, match="does not fit"):
+            opt.load_state_dict(optimizer(bits, ((100, 66), (64,), ()))[0].state_dict())
     with pytest.raises(ValueError):
         opt.load_state_dict(optimizer(32, ((100, 64),))[0].state_dict())
     assert [addresses(opt, p) for p in params] == held
@@ -133,3 +133,21 @@ def test_a_refused_group_is_not_added():
     with pytest.raises(ValueError, match="betas"):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(2))], "betas": (0.9, 1.0)})
     assert len(opt.param_groups) == 1
+
+
+def test_moments_are_converted_one_parameter_at_a_time(monkeypatch):
+    """A checkpoint takes the memory of one parameter's moments beside those that exist, not of all."""
+    opt, params = optimizer(32, ((100, 64), (100, 64), (100, 64)))
+    saved, alive, most = optimizer(8, ((100, 64), (100, 64), (100, 64)))[0].state_dict(), [], []
+    make = FusedAdamW._moments_of
+
+    def watched(self, p, src):
+        st = make(self, p, src)
+        import weakref
+        alive.extend(weakref.ref(t) for k, t in st.items() if k != "step")
+        most.append(sum(r() is not None for r in alive))
+        return st
+
+    monkeypatch.setattr(FusedAdamW, "_moments_of", watched)
+    opt.load_state_dict(saved)
+    assert len(most) == 3 and max(most) <= 4         # this parameter's two, and the last one's still in a variable
