@@ -255,12 +255,18 @@ def torch_ops():
     return _torch_ops
 
 
+def held_by_default_stream(leaf):
+    """Whether a graph from the default stream holds the gradient accumulator of `leaf`: a backward pass over it cannot
+    be recorded then (False where the module that looks is not built)."""
+    return os.path.exists(TORCH_OPS_PATH) and torch_ops().held_by_default_stream(leaf)
+
+
 def stream_ptr(device=None):
     import torch
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-__all__ = ["load", "call", "torch_ops", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "AdamwTensor", "AdamwGroup",
+__all__ = ["load", "call", "torch_ops", "held_by_default_stream", "check", "ptr", "stream_ptr", "SpmmPlan", "DenseReduceJob", "AdamwTensor", "AdamwGroup",
            "RkError", "SIGNATURES",
            "LIB_PATH", "device_count", "require_device", "last_error",
            "c_int32", "c_int64", "c_float", "c_double", "c_uint32", "c_size_t"]

@@ -9,9 +9,11 @@
 // the rest of the package has loaded.  Host code only.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -108,6 +110,21 @@ variable_list only_once(const char *what, variable_list grads) {
   return grads;
 }
 
+// Whether a leaf's gradient would be handed to the default stream: its accumulator remembers the stream that it was made
+// on, and lives as long as some graph over the leaf does.  A stream that records cannot hand anything to the default one.
+bool waits_on_default(torch::autograd::Node *accumulator) {
+  const auto s = accumulator ? accumulator->stream() : std::nullopt;
+  return s && s->id() == c10::hip::getDefaultHIPStream(s->device_index()).id();   // (torch calls its device type CUDA)
+}
+
+void recordable(const char *what, const torch::autograd::Edge &edge) {
+  torch::autograd::Node *next = edge.function.get();
+  if (!dynamic_cast<torch::autograd::AccumulateGrad *>(next) || !waits_on_default(next)) return;
+  TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None, what,
+              ": a backward pass over this leaf cannot be recorded while a graph from the default stream is alive: delete the "
+              "outputs of earlier passes first");
+}
+
 // ---- embedding lookup
 struct LookupBackward : public Node {
   SavedVariable ids_;
@@ -142,6 +159,7 @@ struct LookupBackward : public Node {
     const Tensor &grad = grads[0];
     if (!grad.defined() || !task_should_compute_output(0)) return {Tensor()};
     no_tangent("embedding_lookup", grad);
+    recordable("embedding_lookup", next_edge(0));
     const Tensor ids = ids_.unpack();
     // (linear in the upstream gradient: its derivative matters only where that has one)
     const bool graph = at::GradMode::is_enabled() && grad.requires_grad();
@@ -239,6 +257,7 @@ struct ListBackward : public Node {
     const Tensor g_logps = grads[0].defined() ? grads[0].detach() : Tensor();
     const Tensor g_loss = grads.size() > 1 && grads[1].defined() ? grads[1].detach() : Tensor();
     if ((!g_logps.defined() && !g_loss.defined()) || !task_should_compute_output(0)) return {Tensor()};
+    recordable(what, next_edge(0));
     Tensor scores = scores_.unpack(), items = items_.unpack();
     const bool graph = at::GradMode::is_enabled();
     at::AutoGradMode off(false);
@@ -490,6 +509,11 @@ int64_t adamw_step(const py::list &groups, const py::dict &state, int64_t min_8b
 
 PYBIND11_MODULE(_torch_ops, m) {
   m.def("bind", &bind);
+  m.def("held_by_default_stream", [](const Tensor &leaf) {
+    HANDLE_TH_ERRORS
+    return waits_on_default(torch::autograd::impl::try_get_grad_accumulator(leaf).get());
+    END_HANDLE_TH_ERRORS_PYBIND
+  });
   m.def("embedding_lookup", [](const Tensor &w, const Tensor &ids, double scale, std::optional<int64_t> padding_idx) {
     HANDLE_TH_ERRORS
     return embedding_lookup(w, ids, scale, padding_idx);

@@ -409,7 +409,7 @@ class ShardedTrainStep:
             capture = (self.world == 1 and not dist.is_initialized()) or dist.get_backend(self.group) == "nccl"
         return GraphedStep(self._step, lambda: self.opt.zero_grad(set_to_none=True), example_batch, constants,
                            warmup_steps, capture=capture, capture_error_mode="thread_local",
-                           before_step=getattr(self.opt, "sync_lr", None))
+                           before_step=getattr(self.opt, "sync_lr", None), leaves=self.params)
 
 
 __all__ = ["ShardedGraphConstructor", "ShardedTESTModel", "ShardedTrainStep", "gather_rows"]

@@ -11,11 +11,11 @@ included, with it).
 
 Batches whose size differs from the captured one (the last batch of an epoch) run eagerly.
 """
-from typing import Callable, Dict, Optional
+from typing import Callable, Dict, Iterable, Optional
 
 import torch
 
-from . import ops
+from . import _ffi, ops
 
 UNSAID = object()       # a clipping norm that the caller leaves to the optimizer
 
@@ -41,13 +41,19 @@ class GraphedStep:
     def __init__(self, body: Callable[[Dict], torch.Tensor], zero_grad: Callable[[], None],
                  example_batch: Dict[str, torch.Tensor], constants: Optional[Dict[str, torch.Tensor]] = None,
                  warmup_steps: int = 3, capture: bool = True, capture_error_mode: str = "global",
-                 before_step: Optional[Callable[[], None]] = None):
+                 before_step: Optional[Callable[[], None]] = None, leaves: Iterable[torch.Tensor] = ()):
         """before_step: called before every step behind the capture, outside of it (what the recorded kernels read
-        from device memory and the program keeps on the host: learning rates)."""
+        from device memory and the program keeps on the host: learning rates).
+        leaves: the parameters whose gradients the body accumulates.  One that a graph from the default stream
+        holds (an output of an earlier eager pass that is still alive) cannot be captured over: refused here,
+        where torch ends the process."""
         if warmup_steps < 1:
             # optimizers create their state on the first step; created inside the capture it would
             # be re-zeroed by every replay
             raise ValueError("at least one eager warm-up step is needed before the capture")
+        if capture and any(_ffi.held_by_default_stream(p) for p in leaves):
+            raise RuntimeError("a graph of an earlier pass over these parameters is alive: delete its outputs (losses, scores) "
+                               "before the step is captured")
         self._body_fn, self._zero_grad, self._before_step = body, zero_grad, before_step
         dev = next(iter(example_batch.values())).device
         self.constants = dict(constants or {})
@@ -119,7 +125,7 @@ class GraphedTrainStep(GraphedStep):
         self.params = [p for p in model.parameters() if p.requires_grad]
         # (sync_lr: a rate that a scheduler changed reaches the recorded step)
         super().__init__(self._train_body, lambda: self.opt.zero_grad(set_to_none=True), example_batch, constants,
-                         warmup_steps, before_step=getattr(optimizer, "sync_lr", None))
+                         warmup_steps, before_step=getattr(optimizer, "sync_lr", None), leaves=self.params)
 
     def _train_body(self, batch):
         loss = self.loss_fn(self.model(batch), batch)

@@ -261,3 +261,53 @@ def test_recorded_training_step_follows_a_scheduler(make):
         torch.cuda.synchronize()
         assert torch.equal(net.weight, twin), k
     assert opt.param_groups[0]["lr"] < 0.01
+
+
+def test_a_step_over_leaves_of_a_living_graph_is_not_captured():
+    """Refused before anything is recorded; once the outputs are gone the same step is captured and replayed."""
+    g = torch.Generator().manual_seed(9)
+    net = torch.nn.Module()
+    net.weight = torch.nn.Parameter(torch.randn(64, 8, generator=g).to(DEV))
+    net.forward = lambda b: ops.embedding_lookup(net.weight, b["ids"], padding_idx=0)
+    batch = {"ids": torch.randint(64, (30,), generator=g).to(DEV)}
+    make = lambda: GraphedTrainStep(net, FusedAdamW([net.weight], lr=1e-2), lambda out, b: out.square().mean(), batch)  # noqa: E731
+    out = net(batch)
+    with pytest.raises(RuntimeError, match="delete its outputs"):
+        make()
+    with torch.no_grad():
+        net(batch)
+    del out
+    step, before = make(), net.weight.detach().clone()
+    step(batch)
+    torch.cuda.synchronize()
+    assert not torch.equal(net.weight, before)
+
+
+def test_a_backward_pass_over_a_leaf_of_a_living_graph_is_not_recorded():
+    table, ids, grad, scores, items, ref = inputs(5)
+    table, scores = table.requires_grad_(True), scores.requires_grad_(True)
+    alive = ops.embedding_lookup(table, ids), list_logps(scores, items)
+    side = torch.cuda.Stream()
+    for y, x, up, name in ((lambda: ops.embedding_lookup(table, ids), table, grad, "embedding_lookup"),
+                           (lambda: list_logps(scores, items), scores, torch.ones(8, device=DEV), "list_logps"),
+                           (lambda: preference_loss(scores, items, ref)[0], scores, None, "preference_loss")):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):                    # eagerly it is fine
+            want, = torch.autograd.grad(y(), x, up)
+        torch.cuda.current_stream().wait_stream(side)
+        with pytest.raises(RuntimeError, match=name + ": a backward pass over this leaf cannot be recorded"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                torch.autograd.grad(y(), x, up)
+        torch.cuda.synchronize()
+        assert torch.equal(torch.autograd.grad(y(), x, up)[0], want)
+    del alive
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.embedding_lookup(table, ids), table, grad)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        dw, = torch.autograd.grad(ops.embedding_lookup(table, ids), table, grad)
+    want, = torch.autograd.grad(ops.embedding_lookup(table, ids), table, grad)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dw, want)
