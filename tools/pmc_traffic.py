@@ -1,6 +1,6 @@
 """Summarise the counter passes of tools/pmc_bench.sh.
 
-    python tools/pmc_traffic.py gpurun_out/pmc_bench_<tag> profiles/bench
+    python tools/pmc_traffic.py <folder of the passes> profiles/bench
 
 writes <prefix>_pmc_traffic.json (memory-side bytes per launch of the SpMM hop and of one fused
 top-K call, read by bench.py) and <prefix>_pmc_sq_summary.txt (SQ busy / MFMA-busy / VALU-busy
